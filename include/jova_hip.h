@@ -366,6 +366,82 @@ int jova_scale_dev(const float* x, const float* a_dev, int64_t n, float* y, void
  * buffer; a kernel rather than a memset so that it replays reliably inside a captured hipGraph) */
 int jova_zero(float* p, int64_t n, void* stream);
 
+/* ---- token-sequence operators: no counterpart in the reference; they stand next to its embedding (jova_embedding_*),
+ * recurrence (jova_lstm_*) and optimizer step.  Sequences are time-major [steps, batch, channels] with unit channel
+ * stride; the time and batch strides of inputs are arguments (elements), outputs are dense.  dtype (and weight_dtype): */
+enum { JOVA_F32 = 0, JOVA_BF16 = 1, JOVA_F16 = 2 };
+/* Storage type only: arithmetic, sums and states are fp32 (or wider), results are rounded once.  lengths (optional, DEVICE
+ * int32 [batch], clamped to 0 .. steps): what lies behind a sequence's end is not read, outputs and gradients there are
+ * written as zeros, and the returned state is the one at its end. */
+
+/* out[r][:] = scale * weight[idx[r]][:]; an id outside [0, vocab) sets *bad_flag |= 1 and writes NaN (as jova_embedding_fwd).
+ * Backward: dweight[v][:] = scale * sum over { r : idx[r] = v } of dout[r][:] in ascending r, summed in fp32 and rounded
+ * once (accumulate = 0: every row of dweight is written, rows without a token as zeros; 1: added to what is there, untouched
+ * rows stay).  Rows whose id is padding_idx (-1: none) or outside [0, vocab) add nothing.  No float atomics: the same bits on every call.
+ * n, vocab < 2^31; dweight 16-byte aligned.  workspace (16-byte aligned): the bytes that the function names. */
+int jova_token_embedding_fwd(const void* weight, int dtype, const int64_t* idx, int64_t n, int d, int64_t vocab, float scale,
+                             void* out, int* bad_flag, void* stream);
+size_t jova_token_embedding_bwd_workspace_bytes(int64_t n, int d, int64_t vocab);
+int jova_token_embedding_bwd(const void* dout, int dtype, const int64_t* idx, int64_t n, int d, int64_t vocab,
+                             int64_t padding_idx, float scale, void* dweight, int accumulate, void* workspace, void* stream);
+
+/* Causal depthwise convolution: p[t] = bias + sum_{k<width} weight[:, k] x[t - width + 1 + k], y = p or p * sigmoid(p) (silu);
+ * weight [d, width], width 2 .. 8.  state [width-1, batch, d] (optional, x's type) = the inputs in front of x (zeros without it);
+ * state_out (optional) receives the last width-1 inputs.  Backward: dweight / dbias are written (accumulate = 0) or added to;
+ * dstate_out (optional) = gradient of state_out, dstate (optional) receives that of state.  step: one token a sequence,
+ * x [batch, d] with row stride x_b; state_out may be state (updated in place). */
+int jova_causal_conv_fwd(const void* x, int64_t x_t, int64_t x_b, int dtype, int64_t steps, int64_t batch, int d, int width,
+                         const void* weight, const void* bias_or_null, int weight_dtype, int silu,
+                         const int32_t* lengths_or_null, const void* state_or_null, void* y, void* state_out_or_null,
+                         void* stream);
+size_t jova_causal_conv_bwd_workspace_bytes(int64_t steps, int64_t batch, int d, int width);
+int jova_causal_conv_bwd(const void* x, int64_t x_t, int64_t x_b, const void* dy, int64_t dy_t, int64_t dy_b, int dtype,
+                         int64_t steps, int64_t batch, int d, int width, const void* weight, const void* bias_or_null,
+                         int weight_dtype, int silu, const int32_t* lengths_or_null, const void* state_or_null,
+                         const void* dstate_out_or_null, void* dx, void* dweight, void* dbias_or_null, int accumulate,
+                         void* dstate_or_null, void* workspace, void* stream);
+int jova_causal_conv_step(const void* x, int64_t x_b, const void* state, void* state_out, int dtype, int64_t batch, int d,
+                          int width, const void* weight, const void* bias_or_null, int weight_dtype, int silu, void* y,
+                          void* stream);
+
+/* Selective state space scan: e = dt + dt_bias, or its softplus; h[t] = exp(e A) h[t-1] + e x B; y = (sum_n C h + D x) silu(z).
+ * x, dt, z, dy [steps, batch, d]; B, C [steps, batch, groups, n_state] (the d / groups channels of a group share them);
+ * A [d, n_state], D, dt_bias [d] and the states [batch, d, n_state] are fp32; n_state <= 32.  strides: HOST array of 12 (elements):
+ * time, batch of x, dt, z; time, batch, group of B, C.  state0 (optional) = h in front of the first step, state_out (optional)
+ * = h behind the last.  checkpoints (optional, jova_selective_scan_checkpoint_bytes): states the forward leaves for the backward.
+ * Backward: all gradients are written; dz with z, dD / dbias / dstate0 optional; dB, dC are sums over the group's channels.
+ * step: one token a sequence (x [batch, d], B [batch, groups, n_state]; the time strides are ignored); state_out may be state. */
+size_t jova_selective_scan_checkpoint_bytes(int64_t steps, int64_t batch, int d, int n_state);
+int jova_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
+                            const float* D_or_null, const void* z_or_null, const float* dt_bias_or_null, int dtype,
+                            int64_t steps, int64_t batch, int d, int groups, int n_state, const int64_t* strides,
+                            int softplus, const int32_t* lengths_or_null, const float* state0_or_null, void* y,
+                            float* state_out_or_null, void* checkpoints_or_null, void* stream);
+size_t jova_selective_scan_bwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state);
+int jova_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
+                            const float* D_or_null, const void* z_or_null, const float* dt_bias_or_null, int dtype,
+                            int64_t steps, int64_t batch, int d, int groups, int n_state, const int64_t* strides,
+                            int softplus, const int32_t* lengths_or_null, const void* dy, int64_t dy_t, int64_t dy_b,
+                            const float* dstate_out_or_null, const void* checkpoints, void* dx, void* ddt, void* dz_or_null,
+                            float* dA, void* dB, void* dC, float* dD_or_null, float* dbias_or_null,
+                            float* dstate0_or_null, void* workspace, void* stream);
+int jova_selective_scan_step(const void* x, const void* dt, const float* A, const void* B, const void* C,
+                             const float* D_or_null, const void* z_or_null, const float* dt_bias_or_null, int dtype,
+                             int64_t batch, int d, int groups, int n_state, const int64_t* strides, int softplus,
+                             const float* state, float* state_out, void* y, void* stream);
+
+/* Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_): norm = norm_scale * (sum |g|^kind)^(1/kind) over all
+ * tensors (kind 1, 2; 0 = largest |g|), then out = g * min(1, max_norm / (norm + 1e-6)).  At most JOVA_CLIP_MAX_TENSORS tensors a
+ * call: grads, out, sizes are HOST arrays that travel in the kernel arguments; longer lists make several calls with slots
+ * of their own (jova_grad_norm_slots() doubles each, DEVICE), and every jova_grad_clip call reads all n_slots of them.
+ * out[i] may be grads[i] (in place: nothing is written when the norm is within bounds).  norm_or_null: DEVICE float. */
+#define JOVA_CLIP_MAX_TENSORS 112
+int jova_grad_norm_slots(void);
+int jova_grad_norm(int count, const void* const* grads, const int64_t* sizes, int dtype, int kind, double* slots,
+                   void* stream);
+int jova_grad_clip(int count, const void* const* grads, void* const* out, const int64_t* sizes, int dtype, int kind,
+                   const double* slots, int n_slots, float norm_scale, float max_norm, float* norm_or_null, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,7 @@ import math
 
 import numpy as np
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from .._lib import P, call, ptr_array, stream
@@ -1080,3 +1081,433 @@ class MSELossFunction(torch.autograd.Function):
         g = torch.empty_like(dout)
         call("jova_scale_dev", P(dout), P(_c(dloss.reshape(1).to(dout.dtype))), dout.numel(), P(g), stream())
         return g, None, None
+
+
+# ------------------------------------------------------------------------------------------------------ token sequences
+# Scaled embedding lookup, short causal convolution, selective scan: sequences are time-major [steps, batch, channels] like
+# every sequence here; inputs may be views with any time / batch strides (channels contiguous, else they are copied).
+# These take fp32, bf16 and fp16, run on the device of their inputs and on that device's current stream, and refuse double
+# backward.  lengths: integer tensor [batch] on the same device; steps behind a sequence's end are neither read nor summed.
+_DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _call_on(t, name, *args):
+    """call() with the current stream of the tensor's device appended, under that device."""
+    dev = t.device
+    s = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
+    if dev.index == torch.cuda.current_device():
+        call(name, *args, s)
+    else:
+        with torch.cuda.device(dev):
+            call(name, *args, s)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _unit(t):
+    """t itself when its last dimension is contiguous, else a dense copy."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+def _check_seq(who, ref, **tensors):
+    """Every tensor on the reference's device, in its type where the name does not end in _f32."""
+    if not torch.is_tensor(ref) or ref.dtype not in _DTYPE_CODE:
+        raise TypeError("%s takes float32, bfloat16 or float16 tensors, got %s" % (who, ref.dtype if torch.is_tensor(ref) else type(ref)))
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        want = _F32 if name.endswith("_f32") else ref.dtype
+        if not torch.is_tensor(t) or t.dtype != want:
+            raise TypeError("%s: %s must be a %s tensor, got %s" % (who, name.replace("_f32", ""), want,
+                                                                  t.dtype if torch.is_tensor(t) else type(t)))
+        if t.device != ref.device:
+            raise RuntimeError("%s: %s is on %s, the input on %s" % (who, name.replace("_f32", ""), t.device, ref.device))
+
+
+def _check_shape(who, name, t, shape):
+    if t is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError("%s: %s must be %s, got %s" % (who, name, list(shape), list(t.shape)))
+
+
+def _lengths_i32(who, lengths, x):
+    if lengths is None:
+        return None
+    if not torch.is_tensor(lengths) or lengths.dtype not in (torch.int32, torch.int64):
+        raise TypeError("%s: lengths must be an int32 or int64 tensor" % who)
+    _check_shape(who, "lengths", lengths, (x.shape[1],))
+    if lengths.device != x.device:
+        raise RuntimeError("%s: lengths is on %s, the input on %s" % (who, lengths.device, x.device))
+    if lengths.dtype == torch.int64:
+        lengths = lengths.clamp(0, x.shape[0]).to(torch.int32)
+    return lengths.contiguous()
+
+
+def _grad_slot(param):
+    """(tensor the kernel writes a parameter's gradient to, accumulate, what backward returns): module docstring."""
+    g = param.grad if param.is_leaf else None
+    if g is not None and g.dtype == param.dtype and g.device == param.device and g.is_contiguous() and g.data_ptr() % 16 == 0:
+        return g, 1, None
+    g = torch.empty(param.shape, dtype=param.dtype, device=param.device)
+    return g, 0, g
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _workspace(n, like):
+    return torch.empty(int(n), dtype=torch.uint8, device=like.device)
+
+
+def embedding(idx, weight, scale=1.0, padding_idx=None):
+    """scale * weight[idx] (nn.functional.embedding and a multiplication in one pass).  The gradient is summed per token over
+    the rows sorted by token, in fp32 and in ascending row order: the same bits on every call, unlike EmbeddingFunction's
+    atomics.  Rows equal to padding_idx give no gradient.  An id outside the table yields a NaN row and is reported by
+    EmbeddingFunction.raise_if_bad()."""
+    _check_seq("embedding", weight)
+    if weight.dim() != 2:
+        raise ValueError("embedding: weight must be [tokens, dim], got %s" % (list(weight.shape),))
+    if not torch.is_tensor(idx) or idx.dtype not in (torch.int64, torch.int32):
+        raise TypeError("embedding: idx must be an int64 or int32 tensor")
+    if idx.device != weight.device:
+        raise RuntimeError("embedding: idx is on %s, the table on %s" % (idx.device, weight.device))
+    if weight.shape[1] < 1 or weight.shape[0] < 1:
+        raise ValueError("embedding: empty table %s" % (list(weight.shape),))
+    pad = -1
+    if padding_idx is not None:
+        pad = int(padding_idx)
+        if not -weight.shape[0] <= pad < weight.shape[0]:
+            raise ValueError("embedding: padding_idx %d outside a table of %d" % (pad, weight.shape[0]))
+        pad %= weight.shape[0]
+    _lib.require_gpu(weight)
+    if _wants_grad(weight):
+        if idx.numel() >= 2 ** 31 or weight.shape[0] >= 2 ** 31 - 1:
+            raise ValueError("embedding: the gradient takes fewer than 2^31 rows and tokens")
+        return TokenEmbeddingFunction.apply(weight, idx, float(scale), pad)
+    return _embedding_fwd(idx.to(torch.int64).contiguous(), weight, float(scale))
+
+
+def _bad_flag(device):
+    f = EmbeddingFunction.bad_flag
+    if f is None or f.device != device:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("embedding: run it once on %s before capturing it into a graph (its error flag is made then)" % device)
+        f = EmbeddingFunction.bad_flag = torch.zeros(1, dtype=torch.int32, device=device)
+    return f
+
+
+def _embedding_fwd(idx, weight, scale):
+    w = weight.detach().contiguous()
+    out = torch.empty(tuple(idx.shape) + (w.shape[1],), dtype=w.dtype, device=w.device)
+    _call_on(w, "jova_token_embedding_fwd", _ptr(w), _DTYPE_CODE[w.dtype], _ptr(idx), idx.numel(), w.shape[1], w.shape[0], scale,
+             _ptr(out), _ptr(_bad_flag(w.device)))
+    return out
+
+
+class TokenEmbeddingFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, weight, idx, scale, pad):
+        idx = idx.to(torch.int64).contiguous()
+        ctx.save_for_backward(idx)
+        ctx.param, ctx.scale, ctx.pad = weight, scale, pad
+        return _embedding_fwd(idx, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        (idx,) = ctx.saved_tensors
+        w = ctx.param
+        dw, acc, ret = _grad_slot(w)
+        dout = _c(dout)
+        n, (v, d) = idx.numel(), w.shape
+        ws = _workspace(_lib.lib().jova_token_embedding_bwd_workspace_bytes(n, d, v), dout)
+        _call_on(dout, "jova_token_embedding_bwd", _ptr(dout), _DTYPE_CODE[dout.dtype], _ptr(idx), n, d, v, ctx.pad, ctx.scale,
+                 _ptr(dw), acc, _ptr(ws))
+        return ret, None, None, None
+
+
+def _conv_args(who, x, weight, bias, activation, dims):
+    if not torch.is_tensor(x) or x.dim() != dims:
+        raise ValueError("%s: x must have %d dimensions" % (who, dims))
+    _check_seq(who, x)
+    if weight.dim() != 2 or weight.shape[0] != x.shape[-1] or not 2 <= weight.shape[1] <= 8:
+        raise ValueError("%s: weight must be [%d, 2 .. 8], got %s" % (who, x.shape[-1], list(weight.shape)))
+    if x.shape[-1] < 1:
+        raise ValueError("%s: no channels" % who)
+    if weight.dtype not in (x.dtype, _F32):
+        raise TypeError("%s: weight must be %s or float32, got %s" % (who, x.dtype, weight.dtype))
+    _check_shape(who, "bias", bias, (weight.shape[0],))
+    for name, t in (("weight", weight), ("bias", bias)):
+        if t is not None and t.dtype != weight.dtype:
+            raise TypeError("%s: bias must have the weight's type" % who)
+        if t is not None and t.device != x.device:
+            raise RuntimeError("%s: %s is on %s, the input on %s" % (who, name, t.device, x.device))
+    if activation not in (None, "silu"):
+        raise ValueError("%s: activation must be None or 'silu', got %r" % (who, activation))
+    return int(activation == "silu")
+
+
+def causal_conv1d(x, weight, bias=None, activation=None, lengths=None, initial_state=None, return_final_state=False):
+    """Causal depthwise convolution: y[t] = act(bias + sum_k weight[:, k] x[t - width + 1 + k]) for x [steps, batch, dim],
+    weight [dim, width] (width 2 .. 8; float32 or x's type), activation None or 'silu'.  initial_state [width-1, batch, dim]
+    holds the inputs in front of x (zeros without it).  Returns y, or (y, final_state) for the next piece of the sequence."""
+    who = "causal_conv1d"
+    silu = _conv_args(who, x, weight, bias, activation, 3)
+    _check_seq(who, x, initial_state=initial_state)
+    _check_shape(who, "initial_state", initial_state, (weight.shape[1] - 1, x.shape[1], x.shape[2]))
+    lengths = _lengths_i32(who, lengths, x)
+    _lib.require_gpu(x)
+    if _wants_grad(x, weight, bias, initial_state):
+        y, state = CausalConvFunction.apply(x, weight, bias, initial_state, lengths, silu, bool(return_final_state))
+    else:
+        y, state = _conv_fwd(x, weight, bias, initial_state, lengths, silu, return_final_state)
+    return (y, state) if return_final_state else y
+
+
+def _conv_fwd(x, weight, bias, state, lengths, silu, want_state):
+    x, w, b = _unit(x.detach()), _c(weight.detach()), None if bias is None else _c(bias.detach())
+    state = None if state is None else _c(state.detach())
+    t, n, d = x.shape
+    y = torch.empty((t, n, d), dtype=x.dtype, device=x.device)
+    out = torch.empty((w.shape[1] - 1, n, d), dtype=x.dtype, device=x.device) if want_state else None
+    _call_on(x, "jova_causal_conv_fwd", _ptr(x), x.stride(0), x.stride(1), _DTYPE_CODE[x.dtype], t, n, d, w.shape[1], _ptr(w), _ptr(b),
+             _DTYPE_CODE[w.dtype], silu, _ptr(lengths), _ptr(state), _ptr(y), _ptr(out))
+    return y, out
+
+
+class CausalConvFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, lengths, silu, want_state):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, weight, bias, state, lengths)
+        ctx.params, ctx.silu = (weight, bias), silu
+        return _conv_fwd(x, weight, bias, state, lengths, silu, want_state)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dstate_out):
+        x, weight, bias, state, lengths = ctx.saved_tensors
+        x, w, b, state = _unit(x), _c(weight), None if bias is None else _c(bias), None if state is None else _c(state)
+        t, n, d = x.shape
+        dy = torch.zeros((t, n, d), dtype=x.dtype, device=x.device) if dy is None else _unit(dy)
+        dstate_out = None if dstate_out is None else _c(dstate_out)
+        dx = torch.empty((t, n, d), dtype=x.dtype, device=x.device)
+        dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
+        # both parameter gradients in one way: accumulated in place only where both can be
+        dw, acc, ret_w = _grad_slot(ctx.params[0])
+        db = ret_b = None
+        if bias is not None:
+            db, acc_b, ret_b = _grad_slot(ctx.params[1])
+            if acc_b != acc:
+                dw = ret_w = torch.empty_like(w)
+                db = ret_b = torch.empty_like(b)
+                acc = 0
+        if not ctx.needs_input_grad[1]:
+            dw, ret_w = torch.empty_like(w), None
+        if bias is not None and not ctx.needs_input_grad[2]:
+            db = ret_b = None
+        ws = _workspace(_lib.lib().jova_causal_conv_bwd_workspace_bytes(t, n, d, w.shape[1]), x)
+        _call_on(x, "jova_causal_conv_bwd", _ptr(x), x.stride(0), x.stride(1), _ptr(dy), dy.stride(0), dy.stride(1), _DTYPE_CODE[x.dtype], t, n,
+                 d, w.shape[1], _ptr(w), _ptr(b), _DTYPE_CODE[w.dtype], ctx.silu, _ptr(lengths), _ptr(state), _ptr(dstate_out), _ptr(dx),
+                 _ptr(dw), _ptr(db), acc, _ptr(dstate), _ptr(ws))
+        return dx, ret_w, ret_b, dstate, None, None, None
+
+
+def _out_state(who, state, out_state):
+    """The tensor a single-token call writes the new state to: the old one (in place) or the caller's."""
+    if _wants_grad(state):
+        raise RuntimeError("%s is for inference: the state requires grad" % who)
+    if out_state is None:
+        out_state = state
+    if out_state.shape != state.shape or out_state.dtype != state.dtype or out_state.device != state.device:
+        raise ValueError("%s: out_state must be like state" % who)
+    if not state.is_contiguous() or not out_state.is_contiguous():
+        raise ValueError("%s: state and out_state must be contiguous" % who)
+    if out_state.data_ptr() != state.data_ptr():
+        lo, hi = sorted((state.data_ptr(), out_state.data_ptr()))
+        if state.numel() and hi < lo + state.numel() * state.element_size():
+            raise ValueError("%s: out_state overlaps state without being it" % who)
+    return out_state
+
+
+def causal_conv1d_step(x, state, weight, bias=None, activation=None, out_state=None):
+    """One more input per sequence: x [batch, dim], state [width-1, batch, dim] (causal_conv1d's final state) -> y [batch, dim].
+    The state moves on in place, or into out_state.  Inference only."""
+    who = "causal_conv1d_step"
+    silu = _conv_args(who, x, weight, bias, activation, 2)
+    _check_seq(who, x, state=state)
+    _check_shape(who, "state", state, (weight.shape[1] - 1,) + tuple(x.shape))
+    if _wants_grad(x, weight, bias):
+        raise RuntimeError("%s is for inference: run it under torch.no_grad()" % who)
+    out = _out_state(who, state, out_state)
+    _lib.require_gpu(x)
+    x, w, b = _unit(x), _c(weight), None if bias is None else _c(bias)
+    y = torch.empty(tuple(x.shape), dtype=x.dtype, device=x.device)
+    _call_on(x, "jova_causal_conv_step", _ptr(x), x.stride(0), _ptr(state), _ptr(out), _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1],
+             w.shape[1], _ptr(w), _ptr(b), _DTYPE_CODE[w.dtype], silu, _ptr(y))
+    return y
+
+
+def _scan_check(who, x, dt, A, B, C, D, z, dt_bias):
+    _check_seq(who, x, dt=dt, B=B, C=C, z=z, A_f32=A, D_f32=D, dt_bias_f32=dt_bias)
+    lead, d = tuple(x.shape[:-1]), x.shape[-1]
+    if A.dim() != 2 or A.shape[0] != d or not 1 <= A.shape[1] <= 32:
+        raise ValueError("%s: A must be [%d, 1 .. 32], got %s" % (who, d, list(A.shape)))
+    n = A.shape[1]
+    _check_shape(who, "dt", dt, x.shape)
+    _check_shape(who, "z", z, x.shape)
+    _check_shape(who, "D", D, (d,))
+    _check_shape(who, "dt_bias", dt_bias, (d,))
+    if B.shape != C.shape or tuple(B.shape[:len(lead)]) != lead or B.dim() not in (len(lead) + 1, len(lead) + 2) or B.shape[-1] != n:
+        raise ValueError("%s: B and C must be %s, got %s and %s" % (who, list(lead) + ["groups", n], list(B.shape), list(C.shape)))
+    if B.dim() == len(lead) + 1:
+        B, C = B.unsqueeze(-2), C.unsqueeze(-2)
+    if d < 1 or B.shape[-2] < 1 or d % B.shape[-2] != 0:
+        raise ValueError("%s: %d channels do not divide into %d groups" % (who, d, B.shape[-2]))
+    return B, C
+
+
+def _scan_strides(x, dt, z, B, C):
+    two = lambda t: (t.stride(0), t.stride(1)) if t is not None else (0, 0)                     # noqa: E731
+    return (ctypes.c_int64 * 12)(*two(x), *two(dt), *two(z), *B.stride()[:3], *C.stride()[:3])
+
+
+def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=False, lengths=None, initial_state=None,
+                   return_final_state=False):
+    """Selective state space scan.  x, dt, z [steps, batch, dim]; B, C [steps, batch, groups, n] or [steps, batch, n]; A [dim, n],
+    D and dt_bias [dim] and the states [batch, dim, n] in float32; n <= 32.
+        e = dt + dt_bias (softplus of it with dt_softplus);  h[t] = exp(e A) h[t-1] + e x B;  y = (sum_n C h + D x) silu(z)
+    Returns y, or (y, h behind the last step).  Differentiable in everything but lengths."""
+    who = "selective_scan"
+    if not torch.is_tensor(x) or x.dim() != 3:
+        raise ValueError("%s: x must be [steps, batch, dim]" % who)
+    B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias)
+    _check_seq(who, x, initial_state_f32=initial_state)
+    _check_shape(who, "initial_state", initial_state, (x.shape[1], x.shape[2], A.shape[1]))
+    lengths = _lengths_i32(who, lengths, x)
+    _lib.require_gpu(x)
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
+        y, h = SelectiveScanFunction.apply(x, dt, A, B, C, D, z, dt_bias, initial_state, lengths, bool(dt_softplus), bool(return_final_state))
+    else:
+        y, h, _ = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, initial_state, lengths, dt_softplus, return_final_state, False)
+    return (y, h) if return_final_state else y
+
+
+def _scan_dense(x, dt, A, B, C, D, z, dt_bias):
+    x, dt, z, B, C = (None if t is None else _unit(t.detach()) for t in (x, dt, z, B, C))
+    return (x, dt, _c(A.detach()), B, C, None if D is None else _c(D.detach()), z, None if dt_bias is None else _c(dt_bias.detach()))
+
+
+def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state, want_ckpt):
+    x, dt, A, B, C, D, z, dt_bias = _scan_dense(x, dt, A, B, C, D, z, dt_bias)
+    state = None if state is None else _c(state.detach())
+    (t, b, d), n = x.shape, A.shape[1]
+    y = torch.empty((t, b, d), dtype=x.dtype, device=x.device)
+    h = torch.empty((b, d, n), dtype=_F32, device=x.device) if want_state else None
+    ckpt = _workspace(_lib.lib().jova_selective_scan_checkpoint_bytes(t, b, d, n), x) if want_ckpt else None
+    _call_on(x, "jova_selective_scan_fwd", _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias), _DTYPE_CODE[x.dtype],
+             t, b, d, B.shape[2], n, _scan_strides(x, dt, z, B, C), int(softplus), _ptr(lengths), _ptr(state), _ptr(y), _ptr(h), _ptr(ckpt))
+    return y, h, ckpt
+
+
+class SelectiveScanFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state):
+        ctx.set_materialize_grads(False)
+        y, h, ckpt = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state, True)
+        ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, lengths, ckpt)
+        ctx.softplus = softplus
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh):
+        x, dt, A, B, C, D, z, dt_bias, lengths, ckpt = ctx.saved_tensors
+        x, dt, A, B, C, D, z, dt_bias = _scan_dense(x, dt, A, B, C, D, z, dt_bias)
+        (t, b, d), n, g = x.shape, A.shape[1], B.shape[2]
+        dy = torch.zeros((t, b, d), dtype=x.dtype, device=x.device) if dy is None else _unit(dy)
+        dh = None if dh is None else _c(dh)
+        new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=x.device)                 # noqa: E731
+        new32 = lambda *shape: torch.empty(shape, dtype=_F32, device=x.device)                  # noqa: E731
+        dx, ddt, dz = new(t, b, d), new(t, b, d), new(t, b, d) if z is not None else None
+        dA, dB, dC = new32(d, n), new(t, b, g, n), new(t, b, g, n)
+        dD, dbias = new32(d) if D is not None else None, new32(d) if dt_bias is not None else None
+        dstate = new32(b, d, n) if ctx.needs_input_grad[8] else None
+        ws = _workspace(_lib.lib().jova_selective_scan_bwd_workspace_bytes(t, b, d, g, n), x)
+        _call_on(x, "jova_selective_scan_bwd", _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
+                 _DTYPE_CODE[x.dtype], t, b, d, g, n, _scan_strides(x, dt, z, B, C), int(ctx.softplus), _ptr(lengths), _ptr(dy), dy.stride(0),
+                 dy.stride(1), _ptr(dh), _ptr(ckpt), _ptr(dx), _ptr(ddt), _ptr(dz), _ptr(dA), _ptr(dB), _ptr(dC), _ptr(dD), _ptr(dbias),
+                 _ptr(dstate), _ptr(ws))
+        return dx, ddt, dA, dB, dC, dD, dz, dbias, dstate, None, None, None
+
+
+def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_softplus=False, out_state=None):
+    """One more step per sequence: x, dt, z [batch, dim], B, C [batch, groups, n] or [batch, n], state [batch, dim, n] float32
+    (selective_scan's final state) -> y [batch, dim].  The state moves on in place, or into out_state.  Inference only."""
+    who = "selective_scan_step"
+    if not torch.is_tensor(x) or x.dim() != 2:
+        raise ValueError("%s: x must be [batch, dim]" % who)
+    B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias)
+    _check_seq(who, x, state_f32=state)
+    _check_shape(who, "state", state, tuple(x.shape) + (A.shape[1],))
+    if _wants_grad(x, dt, A, B, C, D, z, dt_bias):
+        raise RuntimeError("%s is for inference: run it under torch.no_grad()" % who)
+    out = _out_state(who, state, out_state)
+    _lib.require_gpu(x)
+    x, dt, A, B, C, D, z, dt_bias = _scan_dense(x, dt, A, B, C, D, z, dt_bias)
+    y = torch.empty(tuple(x.shape), dtype=x.dtype, device=x.device)
+    st = (ctypes.c_int64 * 12)(0, x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), B.stride(1),
+                               0, C.stride(0), C.stride(1))
+    _call_on(x, "jova_selective_scan_step", _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
+             _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], B.shape[1], A.shape[1], st, int(dt_softplus), _ptr(state), _ptr(out), _ptr(y))
+    return y
+
+
+def grad_norm_and_clip(grads, max_norm, kind=2, norm_scale=1.0, out=None):
+    """Global norm of a list of gradient tensors (kind 2, 1, or 0 for the largest magnitude) times norm_scale, and the tensors
+    scaled by min(1, max_norm / (norm + 1e-6)) in place or into ``out`` -> the norm, a float32 device scalar (no host read).
+    Dense tensors of one device; a list of mixed types is summed type by type."""
+    dev = grads[0].device
+    outs = list(grads) if out is None else list(out)
+    if len(outs) != len(grads):
+        raise ValueError("grad clipping: %d outputs for %d tensors" % (len(outs), len(grads)))
+    spans = []
+    for g, o in zip(grads, outs):
+        if g.dtype not in _DTYPE_CODE:
+            raise TypeError("grad clipping takes float32, bfloat16 or float16 tensors, got %s" % g.dtype)
+        if g.device != dev or o.device != dev:
+            raise RuntimeError("grad clipping: all tensors must live on one device")
+        if o.dtype != g.dtype or o.shape != g.shape:
+            raise ValueError("grad clipping: an output must be like its tensor")
+        if not (g.is_contiguous() and o.is_contiguous()):
+            raise ValueError("grad clipping takes contiguous tensors")
+        if o.numel():
+            spans.append((o.data_ptr(), o.numel() * o.element_size()))
+            if o is not g and o.data_ptr() != g.data_ptr():
+                spans.append((g.data_ptr(), g.numel() * g.element_size()))
+    spans.sort()
+    for (p, n), (q, _) in zip(spans, spans[1:]):
+        if q < p + n:
+            raise ValueError("grad clipping: two tensors of the list share memory")
+    _lib.require_gpu(*grads)
+    lib = _lib.lib()
+    slots_each, cap = lib.jova_grad_norm_slots(), 112
+    calls = []
+    for dtype in _DTYPE_CODE:
+        pick = [i for i, g in enumerate(grads) if g.dtype == dtype and g.numel()]
+        for k in range(0, len(pick), cap):
+            ids = pick[k:k + cap]
+            calls.append((dtype, ptr_array([grads[i] for i in ids]), ptr_array([outs[i] for i in ids]),
+                          (ctypes.c_int64 * len(ids))(*[grads[i].numel() for i in ids]), len(ids)))
+    norm = torch.empty((), dtype=_F32, device=dev)
+    if not calls:
+        return norm.zero_()
+    slots = torch.empty(slots_each * len(calls), dtype=torch.float64, device=dev)
+    for k, (dtype, g, _, n, m) in enumerate(calls):
+        _call_on(slots, "jova_grad_norm", m, g, n, _DTYPE_CODE[dtype], kind, slots.data_ptr() + 8 * slots_each * k)
+    for k, (dtype, g, o, n, m) in enumerate(calls):
+        _call_on(slots, "jova_grad_clip", m, g, o, n, _DTYPE_CODE[dtype], kind, _ptr(slots), slots.numel(), float(norm_scale),
+                 float(max_norm), _ptr(norm) if k == 0 else None)
+    return norm

@@ -153,6 +153,42 @@ class Dropout(nn.Dropout):
         return F_.DropoutFunction.apply(x, self.p)
 
 
+class Embedding(nn.Embedding):
+    """nn.Embedding whose rows come out multiplied by ``scale`` and whose gradient is summed per token in a fixed order
+    (functional.embedding).  The options that change the table or the gradient otherwise are refused."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, max_norm=None, scale_grad_by_freq=False,
+                 sparse=False, **kwargs):
+        if max_norm is not None or scale_grad_by_freq or sparse:
+            raise NotImplementedError("Embedding: max_norm, scale_grad_by_freq and sparse are not implemented")
+        super(Embedding, self).__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, **kwargs)
+        self.scale = float(scale)
+
+    def forward(self, x):
+        return F_.embedding(x, self.weight, scale=self.scale, padding_idx=self.padding_idx)
+
+
+class CausalConv1d(nn.Module):
+    """Causal depthwise convolution over [steps, batch, dim] (functional.causal_conv1d); ``step`` takes single tokens."""
+
+    def __init__(self, dim, width=4, bias=True, activation='silu'):
+        super(CausalConv1d, self).__init__()
+        if not 2 <= int(width) <= 8:
+            raise ValueError("CausalConv1d: width must be 2 .. 8, got %r" % (width,))
+        if activation not in (None, 'silu'):
+            raise ValueError("CausalConv1d: activation must be None or 'silu', got %r" % (activation,))
+        self.dim, self.width, self.activation = int(dim), int(width), activation
+        bound = self.width ** -0.5                          # nn.Conv1d(groups=dim)'s own start
+        self.weight = nn.Parameter(torch.empty(self.dim, self.width).uniform_(-bound, bound))
+        self.bias = nn.Parameter(torch.empty(self.dim).uniform_(-bound, bound)) if bias else None
+
+    def forward(self, x, lengths=None, initial_state=None, return_final_state=False):
+        return F_.causal_conv1d(x, self.weight, self.bias, self.activation, lengths, initial_state, return_final_state)
+
+    def step(self, x, state):
+        return F_.causal_conv1d_step(x, state, self.weight, self.bias, self.activation)
+
+
 class ElementwiseBatchNorm(nn.Module):
     """BatchNorm over the last dimension of a tensor of any rank (jova/nn/layers.py:574-588): the tensor is viewed as
     [-1, dim]; the statistics and the normalisation run on the HIP BatchNorm1d."""

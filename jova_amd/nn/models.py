@@ -9,7 +9,7 @@ import torch
 import torch.nn as nn
 
 from . import functional as F_
-from .layers import (BatchNorm1d, Dropout, GraphConvLayer, GraphGather, Linear, ReLU, WeaveBatchNorm, WeaveDropout,
+from .layers import (BatchNorm1d, CausalConv1d, Dropout, Embedding, GraphConvLayer, GraphGather, Linear, ReLU, WeaveBatchNorm, WeaveDropout,
                      WeaveGather, WeaveGather2D, WeaveLayer, get_activation_func)
 
 
@@ -296,6 +296,88 @@ class ProteinRNN(nn.Module):
         m = self.model
         out = F_.LstmFunction.apply(x, m.weight_ih_l0, m.weight_hh_l0, m.bias_ih_l0, m.bias_hh_l0, True)
         return out.permute(1, 0, 2) if self.batch_first else out
+
+
+class ProteinWords(nn.Module):
+    """Word ids of a batch's proteins -> (x [P_max, B, window * dim], segment counts [B]): the input of ProteinSSM.  Takes what
+    Prot2Vec takes; rows come out scaled by sqrt(dim), without an activation, and the table's gradient is summed in a
+    fixed order (layers.Embedding)."""
+
+    def __init__(self, protein_profile, vocab_size, embedding_dim, scale=None):
+        super(ProteinWords, self).__init__()
+        dim = int(embedding_dim)
+        self.protein_profile = protein_profile
+        self.embedding = Embedding(vocab_size + 1, dim, padding_idx=vocab_size, scale=dim ** 0.5 if scale is None else scale)
+        self._table = None
+
+    _resident_table = Prot2Vec._resident_table
+
+    def forward(self, input):
+        w = self.embedding.weight
+        tab = self._resident_table(w.device)
+        off, ln, p_max = input if isinstance(input, tuple) and torch.is_tensor(input[0]) else tab.batch(input, w.device)
+        b, vocab = off.shape[0], self.embedding.num_embeddings - 1
+        idx = torch.empty((b, p_max, tab.window), dtype=torch.int64, device=w.device)
+        out = torch.empty((p_max, b, tab.window), device=w.device)          # (the kernel's values: one column of the table)
+        if p_max:
+            F_.call("jova_prot2vec_fwd", F_.P(tab.table), F_.P(off), F_.P(ln), F_.P(w.detach()), b, p_max, tab.window, 1, vocab, 0,
+                    F_.P(out), F_.P(idx), F_.stream())
+        x = self.embedding(idx.transpose(0, 1))
+        return x.reshape(p_max, b, -1), ln
+
+
+class ProteinSSM(nn.Module):
+    """Selective state space protein encoder, next to ProteinRNN: x [P, B, in_dim] (or ProteinWords' pair with the segment
+    counts) -> relu(out) [P, B, hidden_dim].  in_proj -> (u, gate); u through a short causal convolution with SiLU; x_proj(u)
+    -> time steps, B, C; the scan; out_proj.  No limit on the hidden size, unlike ProteinRNN.  ``step`` extends running
+    sequences by one segment each."""
+
+    def __init__(self, in_dim, hidden_dim, state_dim=16, conv_width=4, expand=2, dt_rank=None, activation='relu'):
+        super(ProteinSSM, self).__init__()
+        if activation != 'relu':
+            raise NotImplementedError("ProteinSSM implements 'relu' (as ProteinRNN)")
+        if not 1 <= int(state_dim) <= 32:
+            raise ValueError("ProteinSSM: state_dim must be 1 .. 32, got %r" % (state_dim,))
+        self.hidden_dim, self.inner, self.state_dim = int(hidden_dim), int(expand) * int(hidden_dim), int(state_dim)
+        self.dt_rank = max(1, self.hidden_dim // 16) if dt_rank is None else int(dt_rank)
+        self.in_proj = Linear(int(in_dim), 2 * self.inner, bias=False)
+        self.conv = CausalConv1d(self.inner, conv_width)
+        self.x_proj = Linear(self.inner, self.dt_rank + 2 * self.state_dim, bias=False)
+        self.dt_proj = Linear(self.dt_rank, self.inner, bias=False)
+        # A = -1 .. -N for every channel; time steps start log-uniform in [1e-3, 1e-1] (softplus of the bias)
+        self.A_log = nn.Parameter(torch.log(torch.arange(1, self.state_dim + 1).float()).repeat(self.inner, 1))
+        start = torch.exp(torch.rand(self.inner) * np.log(100.0) + np.log(1e-3))
+        self.dt_bias = nn.Parameter(start + torch.log(-torch.expm1(-start)))
+        self.D = nn.Parameter(torch.ones(self.inner))
+        self.out_proj = Linear(self.inner, self.hidden_dim)
+
+    def _params(self, u):
+        r, n = self.dt_rank, self.state_dim
+        p = self.x_proj(u)
+        return self.dt_proj(p[..., :r]), -torch.exp(self.A_log), p[..., r:r + n], p[..., r + n:]
+
+    def forward(self, x, lengths=None):
+        if isinstance(x, (tuple, list)):
+            x, lengths = x
+        h = self.in_proj(x)
+        u = self.conv(h[..., :self.inner], lengths=lengths)
+        dt, A, B, C = self._params(u)
+        y = F_.selective_scan(u, dt, A, B, C, D=self.D, z=h[..., self.inner:], dt_bias=self.dt_bias, dt_softplus=True, lengths=lengths)
+        return F_.LinearFunction.apply(y, self.out_proj.weight, self.out_proj.bias, True)
+
+    def new_state(self, batch, device):
+        """Empty running state of ``batch`` sequences for ``step``."""
+        return (torch.zeros(self.conv.width - 1, batch, self.inner, device=device),
+                torch.zeros(batch, self.inner, self.state_dim, device=device))
+
+    def step(self, x, state):
+        """x [B, in_dim], one segment a sequence -> [B, hidden_dim]; ``state`` (new_state) moves on in place."""
+        with torch.no_grad():
+            h = self.in_proj(x)
+            u = self.conv.step(h[..., :self.inner], state[0])
+            dt, A, B, C = self._params(u)
+            y = F_.selective_scan_step(u, dt, A, B, C, state[1], D=self.D, z=h[..., self.inner:], dt_bias=self.dt_bias, dt_softplus=True)
+            return F_.LinearFunction.apply(y, self.out_proj.weight, self.out_proj.bias, True)
 
 
 class ProteinCNN(nn.Module):

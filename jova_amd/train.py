@@ -22,7 +22,7 @@ from .nn import functional as F_
 from .nn.layers import (BatchNorm1d, Dropout, ElementwiseBatchNorm, GraphConvLayer, GraphGather2D, GraphPool, Linear, ReLU,
                         Unsqueeze)
 from .nn.models import (GraphConvSequential, GraphNeuralNet2D, JointAttention, NwayForward, Prot2Vec, ProteinCNN2D,
-                        ProteinRNN)
+                        ProteinRNN, ProteinSSM, ProteinWords)
 
 TUNED_DAVIS_HPARAMS = {
     # first row of proj/dti/soek_res/bayopt_search_integrated_view_attn_no_gan_pcnn2d_ecfp8_gconv_dti_2019_11_27__21_57_05_gp.csv
@@ -60,6 +60,13 @@ def create_prot_net(hparams, model_type, protein_profile):
                              ProteinRNN(in_dim=hparams["prot"]["embedding_dim"] * hparams["prot"]["window"],
                                         hidden_dim=hparams["prot"]["rnn_hidden_state_dim"], dropout=hparams["dprob"],
                                         batch_first=False))
+    if model_type == "ssm":                                         # selective state space encoder (no counterpart there)
+        return nn.Sequential(ProteinWords(protein_profile=protein_profile, vocab_size=hparams["prot"]["vocab_size"],
+                                          embedding_dim=hparams["prot"]["embedding_dim"]),
+                             ProteinSSM(in_dim=hparams["prot"]["embedding_dim"] * hparams["prot"]["window"],
+                                        hidden_dim=hparams["prot"]["ssm_hidden_dim"],
+                                        state_dim=hparams["prot"].get("ssm_state_dim", 16),
+                                        conv_width=hparams["prot"].get("ssm_conv_width", 4)))
     if model_type == "p2v":
         return Prot2Vec(protein_profile=protein_profile, vocab_size=hparams["prot"]["vocab_size"],
                         embedding_dim=hparams["prot"]["embedding_dim"], batch_first=False)
@@ -111,6 +118,8 @@ def create_integrated_net(hparams, protein_profile, c_views=("ecfp8", "gconv"), 
             seg_dims.append(hparams["prot"]["embedding_dim"] * hparams["prot"]["window"])
         elif m_type == "rnn":
             seg_dims.append(hparams["prot"]["rnn_hidden_state_dim"])
+        elif m_type == "ssm":
+            seg_dims.append(hparams["prot"]["ssm_hidden_dim"])
         else:
             seg_dims.append(hparams["prot"]["embedding_dim"])
     layers = [NwayForward(models=views),
@@ -375,6 +384,36 @@ class FlatOptimizer(object):
                       lr, wd, grad_scale, self.step_idx, *[float(v) for v in h], *tail)
 
 
+def clip_grad_norm_(parameters, max_norm, norm_type=2.0, norm_scale=1.0, out=None):
+    """torch.nn.utils.clip_grad_norm_ on the HIP kernels: the norm over all gradients together, the gradients scaled in place
+    by min(1, max_norm / (norm + 1e-6)); returns the norm as a float32 device scalar without reading it on the host.
+
+    ``parameters``: parameters (their ``.grad``; those without one are left out), plain tensors (themselves the gradients) or
+    a single one.  norm_type 2, 1 or inf.  norm_scale multiplies the norm only (1 / world size where the buffer holds the sum
+    over the ranks and the optimizer divides).  ``out``: tensors that receive the clipped gradients, which then stay as
+    they are.  A norm that is not finite makes the gradients so, as in torch."""
+    kinds = {2.0: 2, 1.0: 1, float("inf"): 0}
+    if float(norm_type) not in kinds:
+        raise ValueError("clip_grad_norm_: norm_type must be 1, 2 or inf, got %r" % (norm_type,))
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError("clip_grad_norm_: max_norm must not be negative, got %r" % max_norm)
+    params = [parameters] if torch.is_tensor(parameters) else list(parameters)
+    grads = []
+    for p in params:
+        g = p.grad if isinstance(p, nn.Parameter) or (p.requires_grad and p.is_leaf) else p
+        if g is not None:
+            grads.append(g.detach())
+    if out is not None:
+        out = [out] if torch.is_tensor(out) else list(out)
+    if not grads:
+        if out:
+            raise ValueError("clip_grad_norm_: outputs for no gradient")
+        return torch.zeros((), dtype=torch.float32)
+    with torch.no_grad():
+        return F_.grad_norm_and_clip(grads, max_norm, kinds[float(norm_type)], norm_scale, out)
+
+
 class StepLR(object):
     """torch.optim.lr_scheduler.StepLR over a FlatOptimizer: lr = initial_lr * gamma ** (epoch // step_size).  The
     reference creates StepLR(optimizer, step_size=500, gamma=0.01) and steps it once per epoch
@@ -423,6 +462,10 @@ class Trainer(object):
         self.optimizer.skip_flag = self.nan_flag
         self.optimizer.zero_grads = True
         self.loss_sum = torch.zeros(1, dtype=torch.float32, device=self.flat.data.device)
+        # hparams["max_grad_norm"]: clip the global gradient norm in front of every optimizer step (no counterpart in the
+        # reference, which never clips); grad_norm holds the last step's norm on the device
+        self.max_grad_norm = hparams.get("max_grad_norm")
+        self.grad_norm = None
         self.sync = None
         # (force_sync: run the collectives of the N-rank step on a one-rank group -- rehearsal on a one-GPU box)
         self.collective = world_size > 1 or force_sync
@@ -546,6 +589,8 @@ class Trainer(object):
         lv = loss.detach().reshape(1)
         _lib.call("jova_nonfinite_flag", _lib.P(lv), 1, _lib.P(self.nan_flag), _lib.stream())
         _lib.call("jova_axpy", _lib.P(lv), 1.0, 1, _lib.P(self.loss_sum), _lib.stream())
+        if self.max_grad_norm is not None:
+            self.grad_norm = clip_grad_norm_(self.flat.grad, self.max_grad_norm, norm_scale=scale)
         self.optimizer.step(scale)
         self._grads_clean = bool(self.optimizer.zero_grads)
         return loss, outputs
