@@ -412,11 +412,12 @@ int jova_causal_conv_step(const void* x, int64_t x_b, const void* state, void* s
  * Backward: all gradients are written; dz with z, dD / dbias / dstate0 optional; dB, dC are sums over the group's channels.
  * step: one token a sequence (x [batch, d], B [batch, groups, n_state]; the time strides are ignored); state_out may be state. */
 size_t jova_selective_scan_checkpoint_bytes(int64_t steps, int64_t batch, int d, int n_state);
+size_t jova_selective_scan_fwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state);
 int jova_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
                             const float* D_or_null, const void* z_or_null, const float* dt_bias_or_null, int dtype,
                             int64_t steps, int64_t batch, int d, int groups, int n_state, const int64_t* strides,
                             int softplus, const int32_t* lengths_or_null, const float* state0_or_null, void* y,
-                            float* state_out_or_null, void* checkpoints_or_null, void* stream);
+                            float* state_out_or_null, void* checkpoints_or_null, void* workspace, void* stream);
 size_t jova_selective_scan_bwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state);
 int jova_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
                             const float* D_or_null, const void* z_or_null, const float* dt_bias_or_null, int dtype,

@@ -15,6 +15,7 @@
 namespace {
 
 constexpr int WAVES = 4, CH = 16 * WAVES;              // channels of a workgroup
+constexpr int MAX_CHUNKS = 64, FWD_TARGET = 1024, BWD_TARGET = 512;
 template <int NS> struct Tile { static constexpr int KT = NS <= 4 ? 16 : 8; };      // steps between saved states
 
 struct ScanArgs {
@@ -23,10 +24,11 @@ struct ScanArgs {
     void *y, *dx, *ddt, *dz;
     float *state_out, *dstate0;
     float* ckpt;                                       // [tiles][batch][d][4 NS]: the state in front of every tile
+    float *carry, *esum;                               // [chunks][batch][d][4 NS] and [chunks][batch][d]: carry_in
     float *part_bc, *part_a, *part_d;                  // partial sums of dB | dC, dA, dD | dbias
     const int* lengths;
     long long x_t, x_b, dt_t, dt_b, z_t, z_b, B_t, B_b, B_g, C_t, C_b, C_g, dy_t, dy_b;
-    long long steps;
+    long long steps, chunk;                            // steps of a chunk (blockIdx.z), a multiple of KT
     int batch, d, groups, n, softplus;
 };
 
@@ -67,29 +69,54 @@ __device__ __forceinline__ Where where(const ScanArgs& a) {
     return w;
 }
 
-template <typename T> __device__ __forceinline__ float at_step(const void* p, long long s_t, long long s_b, long long t, const Where& w) {
-    return (p && w.live && t < w.len) ? to_f(((const T*)p)[t * s_t + w.b * s_b + w.ch]) : 0.f;
-}
+// One value per lane: element (t, b, channel) of a [steps, batch, d] tensor.  The part of the address that is the same for the
+// wave stays in scalar registers (base of step t0, advanced by scalar arithmetic), the lane's own part is a 32-bit offset
+// that never changes: strides are checked on the host (LANE_LIMIT).
+template <typename T> struct Lane {
+    const char* base;                                  // of batch element b
+    long long step;                                    // bytes
+    unsigned off;                                      // q * step + channel, bytes
+    __device__ __forceinline__ Lane() {}
+    __device__ __forceinline__ Lane(const void* p, long long s_t, long long s_b, const Where& w)
+        : base((const char*)p + w.b * s_b * (long long)sizeof(T)), step(s_t * (long long)sizeof(T)),
+          off((unsigned)(w.q * s_t + w.ch) * (unsigned)sizeof(T)) {}
+    __device__ __forceinline__ T load(long long t0) const { return *(const T*)(base + t0 * step + off); }
+    __device__ __forceinline__ void store(long long t0, float v) const { *(T*)(const_cast<char*>(base) + t0 * step + off) = from_f<T>(v); }
+};
+// KT / 4 steps of one tensor, as stored; steps behind the end are not touched
+template <typename T, int J> struct Steps {
+    T v[J];
+    __device__ __forceinline__ void load(const Lane<T>& l, bool there, long long t0, long long len, int q) {
+        if (!there) return;
+        if (t0 + 4 * J <= len) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[j] = l.load(t0 + 4 * j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[j] = t0 + 4 * j + q < len ? l.load(t0 + 4 * j) : from_f<T>(0.f);
+        }
+    }
+};
 
 // rows of B and C of KT steps -> LDS, fp32, zero behind the sequence and in the padded states
 template <typename T, int NS>
 struct Rows {
     static constexpr int KT = Tile<NS>::KT, NP = 4 * NS, PER = (2 * KT * NP + 255) / 256;
-    float v[PER];
+    T v[PER];
     __device__ __forceinline__ void load(const ScanArgs& a, const Where& w, long long t0) {
 #pragma unroll
         for (int r = 0; r < PER; ++r) {
             const int i = threadIdx.x + 256 * r, n = i % NP, t = (i / NP) % KT;
-            v[r] = 0.f;
+            v[r] = from_f<T>(0.f);
             if (i >= 2 * KT * NP || n >= a.n || t0 + t >= w.len) continue;
-            v[r] = i < KT * NP ? to_f(((const T*)a.B)[(t0 + t) * a.B_t + w.b * a.B_b + w.g * a.B_g + n])
-                               : to_f(((const T*)a.C)[(t0 + t) * a.C_t + w.b * a.C_b + w.g * a.C_g + n]);
+            v[r] = i < KT * NP ? ((const T*)a.B)[(t0 + t) * a.B_t + w.b * a.B_b + w.g * a.B_g + n]
+                               : ((const T*)a.C)[(t0 + t) * a.C_t + w.b * a.C_b + w.g * a.C_g + n];
         }
     }
     __device__ __forceinline__ void put(float* lds) const {
 #pragma unroll
         for (int r = 0; r < PER; ++r)
-            if (threadIdx.x + 256 * r < 2 * KT * NP) lds[threadIdx.x + 256 * r] = v[r];
+            if (threadIdx.x + 256 * r < 2 * KT * NP) lds[threadIdx.x + 256 * r] = to_f(v[r]);
     }
 };
 
@@ -107,141 +134,289 @@ template <int NS> __device__ __forceinline__ void store_state(float* p, const Sc
         if (p && w.live && n < a.n) p[((long long)w.b * a.d + w.ch) * a.n + n] = h[k];
     }
 }
-template <int NS> __device__ __forceinline__ long long ckpt_at(const ScanArgs& a, const Where& w, long long tile) {
-    return (((tile * a.batch + w.b) * a.d + w.ch) * 4 + w.q) * NS;
+template <int NS> struct alignas(4 * NS) Part { float v[NS]; };
+// a lane's NS states in an array [rows][batch][d][4 NS]
+template <int NS> __device__ __forceinline__ Part<NS>* part_at(float* p, const ScanArgs& a, const Where& w, long long row) {
+    return reinterpret_cast<Part<NS>*>(p) + ((row * a.batch + w.b) * a.d + w.ch) * 4 + w.q;
 }
-
-template <typename T, int NS>
-__global__ void __launch_bounds__(256)
-scan_fwd_kernel(ScanArgs a) {
-    constexpr int KT = Tile<NS>::KT, NP = 4 * NS;
-    __shared__ __align__(16) float rows[2 * KT * NP];
-    const Where w = where(a);
-    const bool b0 = w.q & 1, b1 = w.q & 2;
-    float A2[NS], h[NS];
-    load_state<NS>(a.state0, a, w, h);
+template <int NS> __device__ __forceinline__ void load_A2(const ScanArgs& a, const Where& w, float* A2) {
 #pragma unroll
     for (int k = 0; k < NS; ++k) {
         const int n = w.q * NS + k;
         A2[k] = (w.live && n < a.n) ? a.A[(long long)w.ch * a.n + n] * LOG2E_F : 0.f;
     }
-    const float Dv = (a.D && w.live) ? a.D[w.ch] : 0.f, bias = (a.bias && w.live) ? a.bias[w.ch] : 0.f;
-    Rows<T, NS> next;
-    for (long long t0 = 0; t0 < a.steps; t0 += KT) {
-        next.load(a, w, t0);
-        float x[KT / 4], e[KT / 4], z[KT / 4];
+}
+// The state that enters a chunk: the chunks in front of it (behind it, for the adjoint) are each a product with exp(A sum e)
+// and an addition of what they give from zero.
+template <int NS> __device__ __forceinline__ void carry_in(const ScanArgs& a, const Where& w, const float* A2, int from, int to, int by, float* h) {
+    for (int c = from; c != to; c += by) {
+        const Part<NS> p = *part_at<NS>(a.carry, a, w, c);
+        const float e = a.esum[((long long)c * a.batch + w.b) * a.d + w.ch];
 #pragma unroll
-        for (int j = 0; j < KT / 4; ++j) {
-            const long long t = t0 + 4 * j + w.q;
-            x[j] = at_step<T>(a.x, a.x_t, a.x_b, t, w);
-            const float raw = at_step<T>(a.dt, a.dt_t, a.dt_b, t, w) + bias;
-            e[j] = t < w.len ? (a.softplus ? softplus_f(raw) : raw) : 0.f;
-            z[j] = at_step<T>(a.z, a.z_t, a.z_b, t, w);
+        for (int k = 0; k < NS; ++k) h[k] = fmaf(__builtin_amdgcn_exp2f(e * A2[k]), h[k], p.v[k]);
+    }
+}
+template <typename F> __device__ __forceinline__ void four(F f) {
+    f(std::integral_constant<int, 0>());
+    f(std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 2>());
+    f(std::integral_constant<int, 3>());
+}
+template <typename F> __device__ __forceinline__ void four_back(F f) {
+    f(std::integral_constant<int, 3>());
+    f(std::integral_constant<int, 2>());
+    f(std::integral_constant<int, 1>());
+    f(std::integral_constant<int, 0>());
+}
+
+// LOCAL: the chunk's own contribution to the state (from zero) and its sum of e, for carry_in
+template <typename T, int NS, bool LOCAL>
+__global__ void __launch_bounds__(256)
+scan_fwd_kernel(ScanArgs a) {
+    constexpr int KT = Tile<NS>::KT, NP = 4 * NS, J = KT / 4;
+    __shared__ __align__(16) float rows[2][2 * KT * NP];
+    const Where w = where(a);
+    const bool b0 = w.q & 1, b1 = w.q & 2;
+    const long long first = (long long)blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk);
+    float A2[NS], h[NS], es = 0.f;
+    load_A2<NS>(a, w, A2);
+    if (LOCAL) {
+#pragma unroll
+        for (int k = 0; k < NS; ++k) h[k] = 0.f;
+    } else {
+        load_state<NS>(a.state0, a, w, h);
+        carry_in<NS>(a, w, A2, 0, blockIdx.z, 1, h);
+    }
+    const float Dv = a.D ? a.D[w.ch] : 0.f, bias = a.bias ? a.bias[w.ch] : 0.f;
+    const Lane<T> lx(a.x, a.x_t, a.x_b, w), ldt(a.dt, a.dt_t, a.dt_b, w), lz(a.z, a.z_t, a.z_b, w),
+        ly(a.y, (long long)a.batch * a.d, a.d, w);
+    Rows<T, NS> rn;
+    Steps<T, J> xn, dn, zn;
+    auto fetch = [&](long long t0) {
+        rn.load(a, w, t0);
+        xn.load(lx, true, t0, w.len, w.q);
+        dn.load(ldt, true, t0, w.len, w.q);
+        if (!LOCAL) zn.load(lz, a.z != nullptr, t0, w.len, w.q);
+    };
+    fetch(first);
+    rn.put(rows[0]);
+    __syncthreads();
+    int cur = 0;
+    for (long long t0 = first; t0 < last; t0 += KT, cur ^= 1) {
+        float x[J], e[J], z[J];
+        const bool full = t0 + KT <= w.len;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            x[j] = to_f(xn.v[j]);
+            const float raw = to_f(dn.v[j]) + bias;
+            e[j] = a.softplus ? softplus_f(raw) : raw;
+            if (!LOCAL) z[j] = to_f(zn.v[j]);
         }
-        __syncthreads();                               // the tile before has read its rows
-        next.put(rows);
-        __syncthreads();
-        if (a.ckpt && w.live)
+        if (!full) {
 #pragma unroll
-            for (int k = 0; k < NS; ++k) a.ckpt[ckpt_at<NS>(a, w, t0 / KT) + k] = h[k];
+            for (int j = 0; j < J; ++j)
+                if (t0 + 4 * j + w.q >= w.len) e[j] = 0.f;
+        }
+        if (t0 + KT < last) fetch(t0 + KT);
+        if (!LOCAL && a.ckpt && w.live) {
+            Part<NS> p;
 #pragma unroll
-        for (int j = 0; j < KT / 4; ++j) {
+            for (int k = 0; k < NS; ++k) p.v[k] = h[k];
+            *part_at<NS>(a.ckpt, a, w, t0 / KT) = p;
+        }
+        const float* lds = rows[cur] + w.q * NS;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
             float p[4];
             const float u = e[j] * x[j];
-            auto step = [&](auto ic) {
+            if (LOCAL) es += e[j];
+            four([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const float ei = quad_bcast<i>(e[j]), ui = quad_bcast<i>(u);
-                const float *Bt = rows + (4 * j + i) * NP + w.q * NS, *Ct = Bt + KT * NP;
+                const float *Bt = lds + (4 * j + i) * NP, *Ct = Bt + KT * NP;
                 p[i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
                     h[k] = fmaf(__builtin_amdgcn_exp2f(ei * A2[k]), h[k], ui * Bt[k]);
-                    p[i] = fmaf(Ct[k], h[k], p[i]);
+                    if (!LOCAL) p[i] = fmaf(Ct[k], h[k], p[i]);
                 }
-            };
-            step(std::integral_constant<int, 0>());
-            step(std::integral_constant<int, 1>());
-            step(std::integral_constant<int, 2>());
-            step(std::integral_constant<int, 3>());
-            float y = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
-            if (a.z) y *= z[j] * sigmoid_f(z[j]);
-            const long long t = t0 + 4 * j + w.q;
-            if (w.live && t < a.steps) ((T*)a.y)[(t * a.batch + w.b) * (long long)a.d + w.ch] = from_f<T>(t < w.len ? y : 0.f);
+            });
+            if (!LOCAL) {
+                float y = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
+                if (a.z) y *= z[j] * sigmoid_f(z[j]);
+                const long long t = t0 + 4 * j + w.q;
+                if (w.live && (full || t < a.steps)) ly.store(t0 + 4 * j, full || t < w.len ? y : 0.f);
+            }
+        }
+        if (t0 + KT < last) rn.put(rows[cur ^ 1]);
+        __syncthreads();
+    }
+    if (LOCAL) {
+        es = quad_sum(es);
+        if (!w.live) return;
+        Part<NS> p;
+#pragma unroll
+        for (int k = 0; k < NS; ++k) p.v[k] = h[k];
+        *part_at<NS>(a.carry, a, w, blockIdx.z) = p;
+        if (w.q == 0) a.esum[((long long)blockIdx.z * a.batch + w.b) * a.d + w.ch] = es;
+    } else if (blockIdx.z + 1 == gridDim.z) {
+        store_state<NS>(a.state_out, a, w, h);
+    }
+}
+
+// The adjoint that a chunk hands to the one in front of it, from zero: q <- exp(e A) (q + C g), steps descending
+template <typename T, int NS>
+__global__ void __launch_bounds__(256)
+scan_adjoint_kernel(ScanArgs a) {
+    constexpr int KT = Tile<NS>::KT, NP = 4 * NS, J = KT / 4;
+    __shared__ __align__(16) float rows[2 * KT * NP];
+    const Where w = where(a);
+    const int chunk = blockIdx.z + 1;                  // nothing is in front of chunk 0
+    const long long first = (long long)chunk * a.chunk, last = min(a.steps, first + a.chunk);
+    float A2[NS], q[NS], es = 0.f;
+    load_A2<NS>(a, w, A2);
+#pragma unroll
+    for (int k = 0; k < NS; ++k) q[k] = 0.f;
+    const float bias = a.bias ? a.bias[w.ch] : 0.f;
+    const Lane<T> ldt(a.dt, a.dt_t, a.dt_b, w), lz(a.z, a.z_t, a.z_b, w), ldy(a.dy, a.dy_t, a.dy_b, w);
+    for (long long t0 = first + ((last - first - 1) / KT) * KT; t0 >= first; t0 -= KT) {
+        Rows<T, NS> rn;
+        Steps<T, J> dn, zn, gn;
+        rn.load(a, w, t0);
+        dn.load(ldt, true, t0, w.len, w.q);
+        gn.load(ldy, true, t0, w.len, w.q);
+        zn.load(lz, a.z != nullptr, t0, w.len, w.q);
+        __syncthreads();
+        rn.put(rows);
+        __syncthreads();
+        const float* lds = rows + KT * NP + w.q * NS;
+#pragma unroll
+        for (int j = J - 1; j >= 0; --j) {
+            const float raw = to_f(dn.v[j]) + bias;
+            float e = a.softplus ? softplus_f(raw) : raw, g = to_f(gn.v[j]);
+            if (t0 + 4 * j + w.q >= w.len) e = 0.f;
+            if (a.z) {
+                const float z = to_f(zn.v[j]);
+                g *= z * sigmoid_f(z);
+            }
+            es += e;
+            four_back([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                const float ei = quad_bcast<i>(e), gi = quad_bcast<i>(g);
+                const float* Ct = lds + (4 * j + i) * NP;
+#pragma unroll
+                for (int k = 0; k < NS; ++k) q[k] = fmaf(Ct[k], gi, q[k]) * __builtin_amdgcn_exp2f(ei * A2[k]);
+            });
         }
     }
-    store_state<NS>(a.state_out, a, w, h);
+    es = quad_sum(es);
+    if (!w.live) return;
+    Part<NS> p;
+#pragma unroll
+    for (int k = 0; k < NS; ++k) p.v[k] = q[k];
+    *part_at<NS>(a.carry, a, w, chunk) = p;
+    if (w.q == 0) a.esum[((long long)chunk * a.batch + w.b) * a.d + w.ch] = es;
+}
+
+__device__ __forceinline__ unsigned bits(float v) { return __builtin_bit_cast(unsigned, v); }
+__device__ __forceinline__ float swap32_sum(float a, float b) {        // lanes 0-31: a over both halves, lanes 32-63: b
+    const auto r = __builtin_amdgcn_permlane32_swap(bits(a), bits(b), false, false);
+    const unsigned lo = r[0], hi = r[1];               // (bit_cast of a vector's element reads element 0)
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float swap16_sum(float a, float b) {        // even rows of 16 lanes: a over a pair of rows, odd rows: b
+    const auto r = __builtin_amdgcn_permlane16_swap(bits(a), bits(b), false, false);
+    const unsigned lo = r[0], hi = r[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+// Sums over the wave's 16 channels of v[2][4][NS] (dB | dC, step, state): halved four times, every halving one exchange of
+// lanes and one addition a pair.  Lane l is left with kind l5, step (l4, l3) and the max(NS / 2, 1) states from l2 NS / 2.
+template <int NS> __device__ __forceinline__ void channel_sums(float* v, int lane) {
+#pragma unroll
+    for (int i = 0; i < 4 * NS; ++i) v[i] = swap32_sum(v[i], v[i + 4 * NS]);
+#pragma unroll
+    for (int i = 0; i < 2 * NS; ++i) v[i] = swap16_sum(v[i], v[i + 2 * NS]);
+    const bool l3 = lane & 8, l2 = lane & 4;
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const float lo = v[i] + dpp<0x128>(v[i]), hi = v[i + NS] + dpp<0x128>(v[i + NS]);        // row_ror:8 = the lane with bit 3 flipped
+        v[i] = l3 ? hi : lo;
+    }
+    if (NS == 1) {
+        const float lo = v[0] + dpp<0x104>(v[0]), hi = v[0] + dpp<0x114>(v[0]);                  // row_shl:4, row_shr:4
+        v[0] = l2 ? hi : lo;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NS / 2; ++i) {
+            const float lo = v[i] + dpp<0x104>(v[i]), hi = v[i + NS / 2] + dpp<0x114>(v[i + NS / 2]);
+            v[i] = l2 ? hi : lo;
+        }
+    }
 }
 
 template <typename T, int NS>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, 2)
 scan_bwd_kernel(ScanArgs a) {
-    constexpr int KT = Tile<NS>::KT, NP = 4 * NS;
+    constexpr int KT = Tile<NS>::KT, NP = 4 * NS, J = KT / 4, HALF = NS > 1 ? NS / 2 : 1;
     __shared__ __align__(16) float rows[2 * KT * NP];
-    __shared__ float red[WAVES][KT][2][NP];
+    __shared__ __align__(16) float red[WAVES][KT][2][NP];
     const Where w = where(a);
     const bool b0 = w.q & 1, b1 = w.q & 2;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const long long first = (long long)blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk);
     float A2[NS], q[NS], dA[NS], dD = 0.f, db = 0.f;
+    load_A2<NS>(a, w, A2);
     load_state<NS>(a.dstate_out, a, w, q);
+    carry_in<NS>(a, w, A2, (int)gridDim.z - 1, (int)blockIdx.z, -1, q);
 #pragma unroll
-    for (int k = 0; k < NS; ++k) {
-        const int n = w.q * NS + k;
-        A2[k] = (w.live && n < a.n) ? a.A[(long long)w.ch * a.n + n] * LOG2E_F : 0.f;
-        dA[k] = 0.f;
-    }
-    const float Dv = (a.D && w.live) ? a.D[w.ch] : 0.f, bias = (a.bias && w.live) ? a.bias[w.ch] : 0.f;
-    const int dg_tiles = (a.d / a.groups + CH - 1) / CH;
-    (void)dg_tiles;
-    for (long long tile = (a.steps + KT - 1) / KT - 1; tile >= 0; --tile) {
-        const long long t0 = tile * KT;
-        Rows<T, NS> next;
-        next.load(a, w, t0);
-        float x[KT / 4], e[KT / 4], z[KT / 4], raw[KT / 4], dy[KT / 4], g[KT / 4];
-        float h0[NS], hs[KT][NS], as[KT][NS];
-#pragma unroll
-        for (int k = 0; k < NS; ++k) h0[k] = w.live ? a.ckpt[ckpt_at<NS>(a, w, tile) + k] : 0.f;
-#pragma unroll
-        for (int j = 0; j < KT / 4; ++j) {
-            const long long t = t0 + 4 * j + w.q;
-            x[j] = at_step<T>(a.x, a.x_t, a.x_b, t, w);
-            raw[j] = at_step<T>(a.dt, a.dt_t, a.dt_b, t, w) + bias;
-            e[j] = t < w.len ? (a.softplus ? softplus_f(raw[j]) : raw[j]) : 0.f;
-            z[j] = at_step<T>(a.z, a.z_t, a.z_b, t, w);
-            dy[j] = at_step<T>(a.dy, a.dy_t, a.dy_b, t, w);
-        }
-        next.put(rows);
+    for (int k = 0; k < NS; ++k) dA[k] = 0.f;
+    const float Dv = a.D ? a.D[w.ch] : 0.f, bias = a.bias ? a.bias[w.ch] : 0.f;
+    const long long od_t = (long long)a.batch * a.d;
+    const Lane<T> lx(a.x, a.x_t, a.x_b, w), ldt(a.dt, a.dt_t, a.dt_b, w), lz(a.z, a.z_t, a.z_b, w), ldy(a.dy, a.dy_t, a.dy_b, w);
+    const Lane<T> odx(a.dx, od_t, a.d, w), oddt(a.ddt, od_t, a.d, w), odz(a.dz, od_t, a.d, w);
+    for (long long t0 = first + ((last - first - 1) / KT) * KT; t0 >= first; t0 -= KT) {
+        const bool full = t0 + KT <= w.len;
+        Rows<T, NS> rn;
+        Steps<T, J> xn, dn, zn, gn;
+        rn.load(a, w, t0);
+        const Part<NS> h0 = *part_at<NS>(a.ckpt, a, w, t0 / KT);
+        xn.load(lx, true, t0, w.len, w.q);
+        dn.load(ldt, true, t0, w.len, w.q);
+        gn.load(ldy, true, t0, w.len, w.q);
+        zn.load(lz, a.z != nullptr, t0, w.len, w.q);
+        float x[J], e[J], raw[J], g[J], hs[KT][NS], as[KT][NS];
+        rn.put(rows);
         __syncthreads();
+        const float* lds = rows + w.q * NS;
         // the tile's states once more, and the output in front of the gate
 #pragma unroll
-        for (int j = 0; j < KT / 4; ++j) {
+        for (int j = 0; j < J; ++j) {
+            x[j] = w.live ? to_f(xn.v[j]) : 0.f;
+            raw[j] = to_f(dn.v[j]) + bias;
+            e[j] = a.softplus ? softplus_f(raw[j]) : raw[j];
+            if (!full && t0 + 4 * j + w.q >= w.len) e[j] = 0.f;
+            const float dy = w.live ? to_f(gn.v[j]) : 0.f, u = e[j] * x[j];
             float p[4];
-            const float u = e[j] * x[j];
-            auto step = [&](auto ic) {
+            four([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                const int t = 4 * j + i;
+                const int s = 4 * j + i;
                 const float ei = quad_bcast<i>(e[j]), ui = quad_bcast<i>(u);
-                const float *Bt = rows + t * NP + w.q * NS, *Ct = Bt + KT * NP;
+                const float *Bt = lds + s * NP, *Ct = Bt + KT * NP;
                 p[i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
-                    as[t][k] = __builtin_amdgcn_exp2f(ei * A2[k]);
-                    hs[t][k] = fmaf(as[t][k], t > 0 ? hs[t > 0 ? t - 1 : 0][k] : h0[k], ui * Bt[k]);
-                    p[i] = fmaf(Ct[k], hs[t][k], p[i]);
+                    as[s][k] = __builtin_amdgcn_exp2f(ei * A2[k]);
+                    hs[s][k] = fmaf(as[s][k], s > 0 ? hs[s > 0 ? s - 1 : 0][k] : h0.v[k], ui * Bt[k]);
+                    p[i] = fmaf(Ct[k], hs[s][k], p[i]);
                 }
-            };
-            step(std::integral_constant<int, 0>());
-            step(std::integral_constant<int, 1>());
-            step(std::integral_constant<int, 2>());
-            step(std::integral_constant<int, 3>());
+            });
             const float pre = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
-            g[j] = dy[j];
+            g[j] = dy;
             if (a.z) {
-                const float s = sigmoid_f(z[j]);
-                g[j] = dy[j] * z[j] * s;
+                const float z = to_f(zn.v[j]), sg = sigmoid_f(z);
+                g[j] = dy * z * sg;
                 const long long t = t0 + 4 * j + w.q;
-                if (w.live && t < a.steps)
-                    ((T*)a.dz)[(t * a.batch + w.b) * (long long)a.d + w.ch] =
-                        from_f<T>(t < w.len ? dy[j] * pre * s * (1.f + z[j] * (1.f - s)) : 0.f);
+                if (w.live && (full || t < a.steps)) odz.store(t0 + 4 * j, full || t < w.len ? dy * pre * sg * (1.f + z * (1.f - sg)) : 0.f);
             }
             dD = fmaf(g[j], x[j], dD);
         }
@@ -249,49 +424,42 @@ scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
         for (int k = 0; k < NS; ++k) dAt[k] = 0.f;
 #pragma unroll
-        for (int j = KT / 4 - 1; j >= 0; --j) {
-            float pb[4], pf[4];
+        for (int j = J - 1; j >= 0; --j) {
+            float pb[4], pf[4], v[8 * NS];
             const float u = e[j] * x[j];
-            auto step = [&](auto ic) {
+            four_back([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                const int t = 4 * j + i;
+                const int s = 4 * j + i;
                 const float gi = quad_bcast<i>(g[j]), ui = quad_bcast<i>(u), ei = quad_bcast<i>(e[j]);
-                const float *Bt = rows + t * NP + w.q * NS, *Ct = Bt + KT * NP;
+                const float *Bt = lds + s * NP, *Ct = Bt + KT * NP;
                 pb[i] = pf[i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
                     q[k] = fmaf(Ct[k], gi, q[k]);
                     pb[i] = fmaf(q[k], Bt[k], pb[i]);
-                    float vb = q[k] * ui, vc = gi * hs[t][k];
-                    const float wq = q[k] * as[t][k], f = wq * (t > 0 ? hs[t > 0 ? t - 1 : 0][k] : h0[k]);
+                    v[i * NS + k] = q[k] * ui;
+                    v[(4 + i) * NS + k] = gi * hs[s][k];
+                    q[k] *= as[s][k];
+                    const float f = q[k] * (s > 0 ? hs[s > 0 ? s - 1 : 0][k] : h0.v[k]);
                     dAt[k] = fmaf(f, ei, dAt[k]);
                     pf[i] = fmaf(f, A2[k], pf[i]);
-                    q[k] = wq;
-#pragma unroll
-                    for (int o = 4; o < 64; o <<= 1) {                   // over the wave's 16 channels
-                        vb += __shfl_xor(vb, o, 64);
-                        vc += __shfl_xor(vc, o, 64);
-                    }
-                    if (lane < 4) {
-                        red[wave][t][0][lane * NS + k] = vb;
-                        red[wave][t][1][lane * NS + k] = vc;
-                    }
                 }
-            };
-            step(std::integral_constant<int, 3>());
-            step(std::integral_constant<int, 2>());
-            step(std::integral_constant<int, 1>());
-            step(std::integral_constant<int, 0>());
+            });
+            channel_sums<NS>(v, lane);
+            {
+                float* to = &red[wave][4 * j + ((lane >> 3) & 3)][lane >> 5][w.q * NS + (NS > 1 && (lane & 4) ? NS / 2 : 0)];
+#pragma unroll
+                for (int k = 0; k < HALF; ++k) to[k] = v[k];       // (NS = 1: both lanes write the same sum)
+            }
             const float qb = quad_scatter_sum(pb, b0, b1), fa = quad_scatter_sum(pf, b0, b1) * LN2_F;
             const long long t = t0 + 4 * j + w.q;
             float de = fmaf(qb, x[j], fa);
             if (a.softplus) de *= sigmoid_f(raw[j]);
-            if (t >= w.len) de = 0.f;
+            if (!full && t >= w.len) de = 0.f;
             db += de;
-            if (w.live && t < a.steps) {
-                const long long at = (t * a.batch + w.b) * (long long)a.d + w.ch;
-                ((T*)a.dx)[at] = from_f<T>(t < w.len ? fmaf(g[j], Dv, qb * e[j]) : 0.f);
-                ((T*)a.ddt)[at] = from_f<T>(de);
+            if (w.live && (full || t < a.steps)) {
+                odx.store(t0 + 4 * j, full || t < w.len ? fmaf(g[j], Dv, qb * e[j]) : 0.f);
+                oddt.store(t0 + 4 * j, de);
             }
         }
 #pragma unroll
@@ -306,13 +474,15 @@ scan_bwd_kernel(ScanArgs a) {
                 a.part_bc[((((long long)w.tile * a.steps + t0 + t) * a.batch + w.b) * a.groups + w.g) * 2 * NP + i % (2 * NP)] = s;
         }
     }
-    store_state<NS>(a.dstate0, a, w, q);
+    if (blockIdx.z == 0) store_state<NS>(a.dstate0, a, w, q);
     dD = quad_sum(dD);
     db = quad_sum(db);
     if (w.live) {
-        const long long row = (long long)w.b * a.d + w.ch;
+        const long long row = ((long long)blockIdx.z * a.batch + w.b) * a.d + w.ch;
+        Part<NS> p;
 #pragma unroll
-        for (int k = 0; k < NS; ++k) a.part_a[row * NP + w.q * NS + k] = dA[k];
+        for (int k = 0; k < NS; ++k) p.v[k] = dA[k];
+        reinterpret_cast<Part<NS>*>(a.part_a)[row * 4 + w.q] = p;
         if (w.q == 0) {
             a.part_d[row * 2] = dD;
             a.part_d[row * 2 + 1] = db;
@@ -353,14 +523,17 @@ scan_fold_params_kernel(const float* __restrict__ pa, const float* __restrict__ 
     }
 }
 
+template <typename T> __device__ __forceinline__ float of_token(const void* p, long long s_b, const Where& w) {
+    return p ? to_f(((const T*)p)[w.b * s_b + w.ch]) : 0.f;
+}
 template <typename T, int NS>
 __global__ void __launch_bounds__(256)
 scan_step_kernel(ScanArgs a) {
     const Where w = where(a);
     float h[NS];
     load_state<NS>(a.state0, a, w, h);
-    const float x = at_step<T>(a.x, 0, a.x_b, 0, w), z = at_step<T>(a.z, 0, a.z_b, 0, w);
-    const float raw = at_step<T>(a.dt, 0, a.dt_b, 0, w) + ((a.bias && w.live) ? a.bias[w.ch] : 0.f);
+    const float x = of_token<T>(a.x, a.x_b, w), z = of_token<T>(a.z, a.z_b, w);
+    const float raw = of_token<T>(a.dt, a.dt_b, w) + (a.bias ? a.bias[w.ch] : 0.f);
     const float e = a.softplus ? softplus_f(raw) : raw, u = e * x;
     float p = 0.f;
 #pragma unroll
@@ -420,10 +593,39 @@ ScanArgs scan_args(const void* x, const void* dt, const float* A, const void* B,
     return a;
 }
 
-dim3 scan_grid(const ScanArgs& a) {
-    const int dg = a.d / a.groups;
-    return dim3((unsigned)(a.groups * ((dg + CH - 1) / CH)), (unsigned)a.batch);
+int channel_tiles(int d, int groups) { return groups * ((d / groups + CH - 1) / CH); }
+
+// Chunks of the time axis: enough workgroups to fill the card, few enough that the extra pass over the chunks pays.
+struct Plan { int chunks; long long chunk; };
+Plan scan_plan(int64_t steps, int64_t batch, int d, int groups, int n, int target, int least) {
+    const long long kt = tile_steps(n), wgs = (long long)channel_tiles(d, groups) * batch;
+    Plan p = {1, (steps + kt - 1) / kt * kt};
+    long long c = target / (wgs > 0 ? wgs : 1);
+    if (c > steps / least) c = steps / least;
+    if (c > MAX_CHUNKS) c = MAX_CHUNKS;
+    if (c > 1) {
+        p.chunk = ((steps + c - 1) / c + kt - 1) / kt * kt;
+        p.chunks = (int)((steps + p.chunk - 1) / p.chunk);
+    }
+    if (p.chunk < kt) p.chunk = kt;
+    return p;
 }
+Plan fwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, FWD_TARGET, 128); }
+Plan bwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, BWD_TARGET, 128); }
+
+dim3 scan_grid(const ScanArgs& a, int z = 1) { return dim3((unsigned)channel_tiles(a.d, a.groups), (unsigned)a.batch, (unsigned)z); }
+
+// Lane's 32-bit offsets: 3 steps and a channel, in bytes
+bool lane_ok(const ScanArgs& a) {
+    const long long lim = (1ll << 29);
+    return 3 * a.x_t + a.d < lim && 3 * a.dt_t + a.d < lim && 3 * a.z_t + a.d < lim && 3 * a.dy_t + a.d < lim &&
+           3 * (long long)a.batch * a.d + a.d < lim && a.x_t >= 0 && a.dt_t >= 0 && a.z_t >= 0 && a.dy_t >= 0;
+}
+#define JOVA_SCAN_LANES(who)                                                                    \
+    if (!lane_ok(a)) {                                                                          \
+        jova_set_error(who ": a step of more than 2^29 / 3 elements");                          \
+        return JOVA_ERR_LIMIT;                                                                  \
+    }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
@@ -435,28 +637,59 @@ extern "C" size_t jova_selective_scan_checkpoint_bytes(int64_t steps, int64_t ba
     return (size_t)((steps + kt - 1) / kt) * batch * d * 4 * states_per_lane(n_state) * 4;
 }
 
+extern "C" size_t jova_selective_scan_fwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state) {
+    if (steps <= 0 || batch <= 0 || d < 1 || groups < 1 || n_state < 1 || n_state > 32) return 256;
+    const size_t rows = (size_t)fwd_plan(steps, batch, d, groups, n_state).chunks * batch * d;
+    return align256(rows * 4 * states_per_lane(n_state) * 4) + align256(rows * 4);
+}
+
 extern "C" int jova_selective_scan_fwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
                                        const float* D_or_null, const void* z_or_null, const float* dt_bias_or_null, int dtype,
                                        int64_t steps, int64_t batch, int d, int groups, int n_state, const int64_t* strides,
                                        int softplus, const int32_t* lengths_or_null, const float* state0_or_null, void* y,
-                                       float* state_out_or_null, void* checkpoints_or_null, void* stream) {
+                                       float* state_out_or_null, void* checkpoints_or_null, void* workspace, void* stream) {
     if (const int rc = scan_check("selective_scan_fwd", dtype, steps, batch, d, groups, n_state)) return rc;
-    JOVA_CHECK_ARG(A && strides && (steps * batch == 0 || (x && dt && B && C && y)), "selective_scan_fwd: null pointer");
+    JOVA_CHECK_ARG(A && strides && workspace && (steps * batch == 0 || (x && dt && B && C && y)), "selective_scan_fwd: null pointer");
     if (batch == 0) return JOVA_OK;
     ScanArgs a = scan_args(x, dt, A, B, C, D_or_null, z_or_null, dt_bias_or_null, steps, batch, d, groups, n_state, strides, softplus,
                            lengths_or_null, state0_or_null);
-    a.y = y; a.state_out = state_out_or_null; a.ckpt = (float*)checkpoints_or_null;
+    JOVA_SCAN_LANES("selective_scan_fwd")
+    const Plan p = fwd_plan(steps, batch, d, groups, n_state);
+    a.y = y; a.state_out = state_out_or_null; a.ckpt = (float*)checkpoints_or_null; a.chunk = p.chunk;
+    a.carry = (float*)workspace;
+    a.esum = (float*)((char*)workspace + align256((size_t)p.chunks * batch * d * 4 * states_per_lane(n_state) * 4));
+    const hipStream_t s = (hipStream_t)stream;
     return scan_dispatch(dtype, n_state, [&](auto t, auto k) {
-        hipLaunchKernelGGL((scan_fwd_kernel<decltype(t), decltype(k)::value>), scan_grid(a), dim3(256), 0, (hipStream_t)stream, a);
+        typedef decltype(t) T;
+        constexpr int NS = decltype(k)::value;
+        if (p.chunks > 1) {
+            hipLaunchKernelGGL((scan_fwd_kernel<T, NS, true>), scan_grid(a, p.chunks - 1), dim3(256), 0, s, a);
+            JOVA_CHECK_LAUNCH("selective_scan_fwd (chunks)");
+        }
+        hipLaunchKernelGGL((scan_fwd_kernel<T, NS, false>), scan_grid(a, p.chunks), dim3(256), 0, s, a);
         JOVA_CHECK_LAUNCH("selective_scan_fwd");
         return JOVA_OK;
     });
 }
 
+namespace {
+struct BwdSpace { size_t bc, a, d, carry, esum, all; };
+BwdSpace bwd_space(int64_t steps, int64_t batch, int d, int groups, int n, int chunks) {
+    const size_t np = 4 * states_per_lane(n), rows = (size_t)chunks * batch * d, tiles = (d / groups + CH - 1) / CH;
+    BwdSpace s;
+    s.bc = 0;
+    s.a = s.bc + align256(tiles * steps * batch * groups * 2 * np * 4);
+    s.d = s.a + align256(rows * np * 4);
+    s.carry = s.d + align256(rows * 8);
+    s.esum = s.carry + align256(rows * np * 4);
+    s.all = s.esum + align256(rows * 4);
+    return s;
+}
+}  // namespace
+
 extern "C" size_t jova_selective_scan_bwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state) {
     if (steps < 0 || batch <= 0 || d < 1 || groups < 1 || n_state < 1 || n_state > 32) return 256;
-    const size_t np = 4 * states_per_lane(n_state), tiles = (d / groups + CH - 1) / CH;
-    return align256(tiles * steps * batch * groups * 2 * np * 4) + align256((size_t)batch * d * np * 4) + align256((size_t)batch * d * 8);
+    return bwd_space(steps, batch, d, groups, n_state, bwd_plan(steps, batch, d, groups, n_state).chunks).all;
 }
 
 extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
@@ -472,18 +705,25 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
     JOVA_CHECK_ARG(!z_or_null || dz_or_null, "selective_scan_bwd: z without dz");
     ScanArgs a = scan_args(x, dt, A, B, C, D_or_null, z_or_null, dt_bias_or_null, steps, batch, d, groups, n_state, strides, softplus,
                            lengths_or_null, nullptr);
-    const int np = 4 * states_per_lane(n_state), tiles = (d / groups + CH - 1) / CH;
-    char* ws = (char*)workspace;
-    a.part_bc = (float*)ws;
-    a.part_a = (float*)(ws + align256((size_t)tiles * steps * batch * groups * 2 * np * 4));
-    a.part_d = (float*)((char*)a.part_a + align256((size_t)batch * d * np * 4));
     a.dy = dy; a.dy_t = dy_t; a.dy_b = dy_b; a.dstate_out = dstate_out_or_null; a.ckpt = (float*)checkpoints;
+    JOVA_SCAN_LANES("selective_scan_bwd")
+    const int np = 4 * states_per_lane(n_state), tiles = (d / groups + CH - 1) / CH;
+    const Plan p = bwd_plan(steps, batch, d, groups, n_state);
+    const BwdSpace sp = bwd_space(steps, batch, d, groups, n_state, p.chunks);
+    char* ws = (char*)workspace;
+    a.part_bc = (float*)(ws + sp.bc); a.part_a = (float*)(ws + sp.a); a.part_d = (float*)(ws + sp.d);
+    a.carry = (float*)(ws + sp.carry); a.esum = (float*)(ws + sp.esum); a.chunk = p.chunk;
     a.dx = dx; a.ddt = ddt; a.dz = dz_or_null; a.dstate0 = dstate0_or_null;
     const hipStream_t s = (hipStream_t)stream;
     if (batch > 0) {
         const int rc = scan_dispatch(dtype, n_state, [&](auto t, auto k) {
             typedef decltype(t) T;
-            hipLaunchKernelGGL((scan_bwd_kernel<T, decltype(k)::value>), scan_grid(a), dim3(256), 0, s, a);
+            constexpr int NS = decltype(k)::value;
+            if (p.chunks > 1) {
+                hipLaunchKernelGGL((scan_adjoint_kernel<T, NS>), scan_grid(a, p.chunks - 1), dim3(256), 0, s, a);
+                JOVA_CHECK_LAUNCH("selective_scan_bwd (chunks)");
+            }
+            hipLaunchKernelGGL((scan_bwd_kernel<T, NS>), scan_grid(a, p.chunks), dim3(256), 0, s, a);
             JOVA_CHECK_LAUNCH("selective_scan_bwd");
             const long long rows = (long long)steps * batch * groups, total = rows * 2 * np;
             if (total) {
@@ -496,8 +736,8 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
         if (rc) return rc;
     }
     const long long cols = (long long)d * (np + 2);
-    hipLaunchKernelGGL(scan_fold_params_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, s, a.part_a, a.part_d, (int)batch, d, np,
-                       n_state, dA, dD_or_null, dbias_or_null);
+    hipLaunchKernelGGL(scan_fold_params_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, s, a.part_a, a.part_d,
+                       (int)(batch * p.chunks), d, np, n_state, dA, dD_or_null, dbias_or_null);
     JOVA_CHECK_LAUNCH("selective_scan_bwd (parameters)");
     return JOVA_OK;
 }

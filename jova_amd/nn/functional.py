@@ -1407,8 +1407,10 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_stat
     y = torch.empty((t, b, d), dtype=x.dtype, device=x.device)
     h = torch.empty((b, d, n), dtype=_F32, device=x.device) if want_state else None
     ckpt = _workspace(_lib.lib().jova_selective_scan_checkpoint_bytes(t, b, d, n), x) if want_ckpt else None
+    ws = _workspace(_lib.lib().jova_selective_scan_fwd_workspace_bytes(t, b, d, B.shape[2], n), x)
     _call_on(x, "jova_selective_scan_fwd", _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias), _DTYPE_CODE[x.dtype],
-             t, b, d, B.shape[2], n, _scan_strides(x, dt, z, B, C), int(softplus), _ptr(lengths), _ptr(state), _ptr(y), _ptr(h), _ptr(ckpt))
+             t, b, d, B.shape[2], n, _scan_strides(x, dt, z, B, C), int(softplus), _ptr(lengths), _ptr(state), _ptr(y), _ptr(h), _ptr(ckpt),
+             _ptr(ws))
     return y, h, ckpt
 
 

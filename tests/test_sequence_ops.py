@@ -104,8 +104,8 @@ def test_abi_refusals_without_a_gpu():
         ("jova_causal_conv_fwd", (p, 8, 8, 0, 4, 70000, 8, 4, p, p, 0, 1, None, None, p, None, None), "65535"),
         ("jova_causal_conv_bwd", (p, 8, 8, p, 8, 8, 0, 4, 2, 8, 4, p, p, 3, 1, None, None, None, p, p, p, 0, None, p, None), "dtype"),
         ("jova_causal_conv_step", (p, 8, None, p, 0, 2, 8, 4, p, p, 0, 1, p, None), "null pointer"),
-        ("jova_selective_scan_fwd", (p, p, p, p, p, p, p, p, 0, 4, 2, 8, 3, 16, n8, 1, None, None, p, None, None, None), "bad shape"),
-        ("jova_selective_scan_fwd", (p, p, p, p, p, p, p, p, 0, 4, 2, 8, 1, 33, n8, 1, None, None, p, None, None, None), "at most 32"),
+        ("jova_selective_scan_fwd", (p, p, p, p, p, p, p, p, 0, 4, 2, 8, 3, 16, n8, 1, None, None, p, None, None, p, None), "bad shape"),
+        ("jova_selective_scan_fwd", (p, p, p, p, p, p, p, p, 0, 4, 2, 8, 1, 33, n8, 1, None, None, p, None, None, p, None), "at most 32"),
         ("jova_selective_scan_step", (p, p, p, p, p, p, p, p, 0, 2, 8, 1, 16, n8, 1, None, p, p, None), "null pointer"),
         ("jova_grad_norm", (113, p, p, 0, 2, p, None), "tensors a call"),
         ("jova_grad_norm", (1, p, p, 0, 3, p, None), "norm kind"),
