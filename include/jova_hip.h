@@ -432,16 +432,13 @@ int jova_selective_scan_step(const void* x, const void* dt, const float* A, cons
                              const float* state, float* state_out, void* y, void* stream);
 
 /* Global gradient norm and clipping (torch.nn.utils.clip_grad_norm_): norm = norm_scale * (sum |g|^kind)^(1/kind) over all
- * tensors (kind 1, 2; 0 = largest |g|), then out = g * min(1, max_norm / (norm + 1e-6)).  At most JOVA_CLIP_MAX_TENSORS tensors a
- * call: grads, out, sizes are HOST arrays that travel in the kernel arguments; longer lists make several calls with slots
- * of their own (jova_grad_norm_slots() doubles each, DEVICE), and every jova_grad_clip call reads all n_slots of them.
- * out[i] may be grads[i] (in place: nothing is written when the norm is within bounds).  norm_or_null: DEVICE float. */
-#define JOVA_CLIP_MAX_TENSORS 112
-int jova_grad_norm_slots(void);
-int jova_grad_norm(int count, const void* const* grads, const int64_t* sizes, int dtype, int kind, double* slots,
-                   void* stream);
-int jova_grad_clip(int count, const void* const* grads, void* const* out, const int64_t* sizes, int dtype, int kind,
-                   const double* slots, int n_slots, float norm_scale, float max_norm, float* norm_or_null, void* stream);
+ * tensors (kind 1, 2; 0 = largest |g|), then out = g * min(1, max_norm / (norm + 1e-6)).  grads, out, sizes (elements), dtypes:
+ * HOST arrays of `count`, read before the call returns (they travel in the kernel arguments); two launches per type and 112
+ * tensors.  out[i] may be grads[i] (in place: nothing is written when the norm is within bounds); apart from that no two
+ * tensors may share memory (an error).  norm: DEVICE float.  workspace: DEVICE, the bytes that the function names. */
+size_t jova_clip_grads_workspace_bytes(int count);
+int jova_clip_grads(int count, const void* const* grads, void* const* out, const int64_t* sizes, const int32_t* dtypes,
+                    int kind, float norm_scale, float max_norm, float* norm, void* workspace, void* stream);
 
 #ifdef __cplusplus
 }

@@ -70,8 +70,7 @@ _SIGS = {
     "jova_selective_scan_fwd": "pppppppp" + "iqqiiip" + "ippp" + "pppp",
     "jova_selective_scan_bwd": "pppppppp" + "iqqiiip" + "ip" + "pqqpp" + "ppp" + "pppppp" + "pp",
     "jova_selective_scan_step": "pppppppp" + "iqiiipi" + "pppp",
-    "jova_grad_norm": "ippiipp",
-    "jova_grad_clip": "ipppii" + "piffpp",
+    "jova_clip_grads": "ipppp" + "iff" + "ppp",
 }
 _CT = {"p": ctypes.c_void_p, "i": ctypes.c_int, "q": ctypes.c_int64, "f": ctypes.c_float, "Q": ctypes.c_uint64,
        "d": ctypes.c_double}
@@ -81,7 +80,7 @@ EXPORTS = sorted(list(_SIGS) + ["jova_last_error", "jova_abi_version", "jova_non
                                 "jova_nonsat_set_spin_limit", "jova_nonsat_noalloc_max_n", "jova_gemm_set_bf16x3", "jova_gemm_get_bf16x3",
                                 "jova_gemm_b_image_bytes", "jova_token_embedding_bwd_workspace_bytes",
                                 "jova_causal_conv_bwd_workspace_bytes", "jova_selective_scan_checkpoint_bytes",
-                                "jova_selective_scan_fwd_workspace_bytes", "jova_selective_scan_bwd_workspace_bytes", "jova_grad_norm_slots"])
+                                "jova_selective_scan_fwd_workspace_bytes", "jova_selective_scan_bwd_workspace_bytes", "jova_clip_grads_workspace_bytes"])
 
 _lib = None
 
@@ -118,13 +117,12 @@ def lib():
         L.jova_gemm_b_image_bytes.restype = ctypes.c_size_t
         L.jova_gemm_b_image_bytes.argtypes = [_CT[c] for c in "pqqpqqiiiiii"]
         for name, sig in (("jova_token_embedding_bwd_workspace_bytes", "qiq"), ("jova_causal_conv_bwd_workspace_bytes", "qqii"),
+                          ("jova_clip_grads_workspace_bytes", "i"),
                           ("jova_selective_scan_checkpoint_bytes", "qqii"),
                           ("jova_selective_scan_fwd_workspace_bytes", "qqiii"),
                           ("jova_selective_scan_bwd_workspace_bytes", "qqiii")):
             getattr(L, name).restype = ctypes.c_size_t
             getattr(L, name).argtypes = [_CT[c] for c in sig]
-        L.jova_grad_norm_slots.restype = ctypes.c_int
-        L.jova_grad_norm_slots.argtypes = []
         _lib = L
     return _lib
 

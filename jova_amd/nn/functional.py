@@ -1470,46 +1470,33 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
 def grad_norm_and_clip(grads, max_norm, kind=2, norm_scale=1.0, out=None):
     """Global norm of a list of gradient tensors (kind 2, 1, or 0 for the largest magnitude) times norm_scale, and the tensors
     scaled by min(1, max_norm / (norm + 1e-6)) in place or into ``out`` -> the norm, a float32 device scalar (no host read).
-    Dense tensors of one device; a list of mixed types is summed type by type."""
-    dev = grads[0].device
-    outs = list(grads) if out is None else list(out)
-    if len(outs) != len(grads):
-        raise ValueError("grad clipping: %d outputs for %d tensors" % (len(outs), len(grads)))
-    spans = []
-    for g, o in zip(grads, outs):
-        if g.dtype not in _DTYPE_CODE:
-            raise TypeError("grad clipping takes float32, bfloat16 or float16 tensors, got %s" % g.dtype)
-        if g.device != dev or o.device != dev:
-            raise RuntimeError("grad clipping: all tensors must live on one device")
-        if o.dtype != g.dtype or o.shape != g.shape:
-            raise ValueError("grad clipping: an output must be like its tensor")
-        if not (g.is_contiguous() and o.is_contiguous()):
-            raise ValueError("grad clipping takes contiguous tensors")
-        if o.numel():
-            spans.append((o.data_ptr(), o.numel() * o.element_size()))
-            if o is not g and o.data_ptr() != g.data_ptr():
-                spans.append((g.data_ptr(), g.numel() * g.element_size()))
-    spans.sort()
-    for (p, n), (q, _) in zip(spans, spans[1:]):
-        if q < p + n:
-            raise ValueError("grad clipping: two tensors of the list share memory")
-    _lib.require_gpu(*grads)
-    lib = _lib.lib()
-    slots_each, cap = lib.jova_grad_norm_slots(), 112
-    calls = []
-    for dtype in _DTYPE_CODE:
-        pick = [i for i, g in enumerate(grads) if g.dtype == dtype and g.numel()]
-        for k in range(0, len(pick), cap):
-            ids = pick[k:k + cap]
-            calls.append((dtype, ptr_array([grads[i] for i in ids]), ptr_array([outs[i] for i in ids]),
-                          (ctypes.c_int64 * len(ids))(*[grads[i].numel() for i in ids]), len(ids)))
-    norm = torch.empty((), dtype=_F32, device=dev)
-    if not calls:
-        return norm.zero_()
-    slots = torch.empty(slots_each * len(calls), dtype=torch.float64, device=dev)
-    for k, (dtype, g, _, n, m) in enumerate(calls):
-        _call_on(slots, "jova_grad_norm", m, g, n, _DTYPE_CODE[dtype], kind, slots.data_ptr() + 8 * slots_each * k)
-    for k, (dtype, g, o, n, m) in enumerate(calls):
-        _call_on(slots, "jova_grad_clip", m, g, o, n, _DTYPE_CODE[dtype], kind, _ptr(slots), slots.numel(), float(norm_scale),
-                 float(max_norm), _ptr(norm) if k == 0 else None)
+    Contiguous tensors of one device, types may be mixed; an output has its tensor's type and element count."""
+    who, n = "grad clipping", len(grads)
+    outs = grads if out is None else out
+    if len(outs) != n:
+        raise ValueError("%s: %d outputs for %d tensors" % (who, len(outs), n))
+    try:
+        codes = [_DTYPE_CODE[g.dtype] for g in grads]
+    except KeyError as e:
+        raise TypeError("%s takes float32, bfloat16 or float16 tensors, got %s" % (who, e)) from None
+    sizes = [g.numel() for g in grads]
+    devs = {g.get_device() for g in grads}
+    dense = all([g.is_contiguous() for g in grads])
+    gp = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
+    op = gp
+    if outs is not grads:
+        if [o.numel() for o in outs] != sizes or [o.dtype for o in outs] != [g.dtype for g in grads]:
+            raise ValueError("%s: an output must have its tensor's type and element count" % who)
+        devs |= {o.get_device() for o in outs}
+        dense = dense and all([o.is_contiguous() for o in outs])
+        op = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+    if not dense:
+        raise ValueError("%s takes contiguous tensors" % who)
+    if len(devs) != 1:
+        raise RuntimeError("%s: all tensors must live on one device" % who)
+    _lib.require_gpu(grads[0])
+    norm = torch.empty((), dtype=_F32, device=grads[0].device)
+    ws = _workspace(_lib.lib().jova_clip_grads_workspace_bytes(n), norm)
+    _call_on(norm, "jova_clip_grads", n, gp, op, (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*codes), kind, float(norm_scale),
+             float(max_norm), norm.data_ptr(), ws.data_ptr())
     return norm

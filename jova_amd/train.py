@@ -399,19 +399,15 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, norm_scale=1.0, out=Non
     if not max_norm >= 0.0:
         raise ValueError("clip_grad_norm_: max_norm must not be negative, got %r" % max_norm)
     params = [parameters] if torch.is_tensor(parameters) else list(parameters)
-    grads = []
-    for p in params:
-        g = p.grad if isinstance(p, nn.Parameter) or (p.requires_grad and p.is_leaf) else p
-        if g is not None:
-            grads.append(g.detach())
+    grads = [p.grad if isinstance(p, nn.Parameter) or (p.requires_grad and p.is_leaf) else p for p in params]
+    grads = [g for g in grads if g is not None]
     if out is not None:
         out = [out] if torch.is_tensor(out) else list(out)
     if not grads:
         if out:
             raise ValueError("clip_grad_norm_: outputs for no gradient")
         return torch.zeros((), dtype=torch.float32)
-    with torch.no_grad():
-        return F_.grad_norm_and_clip(grads, max_norm, kinds[float(norm_type)], norm_scale, out)
+    return F_.grad_norm_and_clip(grads, max_norm, kinds[float(norm_type)], norm_scale, out)
 
 
 class StepLR(object):

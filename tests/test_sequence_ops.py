@@ -95,6 +95,8 @@ def test_scan_restatement_against_autograd_and_differences(gate):
 def test_abi_refusals_without_a_gpu():
     from jova_amd import _lib
     p, n8 = ctypes.c_void_p(4096), (ctypes.c_int64 * 12)()
+    one, two = (ctypes.c_void_p * 1)(4096), (ctypes.c_void_p * 2)(4096, 4100)
+    size, code = (ctypes.c_int64 * 2)(8, 8), (ctypes.c_int32 * 2)(0, 0)
     bad = [
         ("jova_token_embedding_fwd", (p, 7, p, 4, 8, 10, 1.0, p, p, None), "dtype"),
         ("jova_token_embedding_fwd", (None, 0, p, 4, 8, 10, 1.0, p, p, None), "bad argument"),
@@ -107,8 +109,10 @@ def test_abi_refusals_without_a_gpu():
         ("jova_selective_scan_fwd", (p, p, p, p, p, p, p, p, 0, 4, 2, 8, 3, 16, n8, 1, None, None, p, None, None, p, None), "bad shape"),
         ("jova_selective_scan_fwd", (p, p, p, p, p, p, p, p, 0, 4, 2, 8, 1, 33, n8, 1, None, None, p, None, None, p, None), "at most 32"),
         ("jova_selective_scan_step", (p, p, p, p, p, p, p, p, 0, 2, 8, 1, 16, n8, 1, None, p, p, None), "null pointer"),
-        ("jova_grad_norm", (113, p, p, 0, 2, p, None), "tensors a call"),
-        ("jova_grad_norm", (1, p, p, 0, 3, p, None), "norm kind"),
+        ("jova_clip_grads", (1, one, one, size, code, 3, 1.0, 1.0, p, p, None), "norm kind"),
+        ("jova_clip_grads", (0, one, one, size, code, 2, 1.0, 1.0, p, p, None), "bad argument"),
+        ("jova_clip_grads", (1, one, one, size, (ctypes.c_int32 * 1)(5), 2, 1.0, 1.0, p, p, None), "dtype"),
+        ("jova_clip_grads", (2, two, two, size, code, 2, 1.0, 1.0, p, p, None), "share memory"),
     ]
     for name, args, text in bad:
         with pytest.raises(RuntimeError, match=text):
@@ -152,7 +156,6 @@ def test_python_refusals_without_a_gpu():
         (lambda: F.selective_scan_step(out_state=torch.zeros(2, 4, 4), **one), dict(error=ValueError)),
         (lambda: clip_grad_norm_([w], 1.0), G), (lambda: clip_grad_norm_([w], 1.0, norm_type=3), dict(error=ValueError)),
         (lambda: clip_grad_norm_([w], -1.0), dict(error=ValueError)), (lambda: clip_grad_norm_([w], float("nan")), dict(error=ValueError)),
-        (lambda: clip_grad_norm_([w, w], 1.0), dict(error=ValueError, match="share memory")),
         (lambda: clip_grad_norm_([w[:, :2]], 1.0), dict(error=ValueError, match="contiguous")),
         (lambda: clip_grad_norm_([w.double()], 1.0), dict(error=TypeError)),
         (lambda: clip_grad_norm_([w], 1.0, out=[w[:5]]), dict(error=ValueError)),
@@ -534,6 +537,14 @@ def test_clip_norm_and_scaling(device, sizes, kind):
 @pytest.mark.gpu
 def test_clip_extremes(device):
     from jova_amd.train import clip_grad_norm_
+    w = torch.ones(100, device=device)
+    for lists in (([w, w], None), ([w[:60], w[40:]], None), ([w[:50]], [w[10:60]])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            clip_grad_norm_(lists[0], 1.0, out=lists[1])
+    odd = torch.arange(40000, device=device, dtype=torch.float32)[1:].sub_(20000.0)           # not on a 16-byte boundary
+    want = odd.double().norm()
+    clip_grad_norm_([odd], 1.0)
+    assert abs(float(odd.double().norm()) - 1.0) <= 1e-6 and float(want) > 1e6
     big = torch.full((1000,), 3e38, device=device)
     keep = big.clone()
     n = clip_grad_norm_([big[:1]], 1.0)
