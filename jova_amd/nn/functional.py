@@ -1091,15 +1091,23 @@ class MSELossFunction(torch.autograd.Function):
 _DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_FN = {}
+
+
 def _call_on(t, name, *args):
-    """call() with the current stream of the tensor's device appended, under that device."""
-    dev = t.device
-    s = ctypes.c_void_p(torch.cuda.current_stream(dev).cuda_stream)
-    if dev.index == torch.cuda.current_device():
-        call(name, *args, s)
+    """call() with the current stream of the tensor's device appended, under that device.  (The single-token calls are bound by
+    the host: raw stream handle, bound functions kept.)"""
+    fn = _FN.get(name)
+    if fn is None:
+        fn = _FN[name] = getattr(_lib.lib(), name)
+    dev = t.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            call(name, *args, s)
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc != 0:
+        raise RuntimeError("%s failed (%d): %s" % (name, rc, _lib.lib().jova_last_error().decode()))
 
 
 def _ptr(t):
@@ -1111,23 +1119,28 @@ def _unit(t):
     return t if t is None or t.stride(-1) == 1 else t.contiguous()
 
 
-def _check_seq(who, ref, **tensors):
-    """Every tensor on the reference's device, in its type where the name does not end in _f32."""
-    if not torch.is_tensor(ref) or ref.dtype not in _DTYPE_CODE:
+def _c_opt(t):
+    return t if t is None or t.is_contiguous() else t.contiguous()
+
+
+def _check_type(who, name, t, dtype, ref):
+    if t is None:
+        return
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError("%s: %s must be a %s tensor, got %s" % (who, name, dtype, t.dtype if torch.is_tensor(t) else type(t)))
+    if t.get_device() != ref.get_device():
+        raise RuntimeError("%s: %s is on %s, the input on %s" % (who, name, t.device, ref.device))
+
+
+def _check_input(who, ref, dims):
+    if not isinstance(ref, torch.Tensor) or ref.dtype not in _DTYPE_CODE:
         raise TypeError("%s takes float32, bfloat16 or float16 tensors, got %s" % (who, ref.dtype if torch.is_tensor(ref) else type(ref)))
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        want = _F32 if name.endswith("_f32") else ref.dtype
-        if not torch.is_tensor(t) or t.dtype != want:
-            raise TypeError("%s: %s must be a %s tensor, got %s" % (who, name.replace("_f32", ""), want,
-                                                                  t.dtype if torch.is_tensor(t) else type(t)))
-        if t.device != ref.device:
-            raise RuntimeError("%s: %s is on %s, the input on %s" % (who, name.replace("_f32", ""), t.device, ref.device))
+    if ref.dim() != dims:
+        raise ValueError("%s: x must have %d dimensions, got %s" % (who, dims, list(ref.shape)))
 
 
 def _check_shape(who, name, t, shape):
-    if t is not None and tuple(t.shape) != tuple(shape):
+    if t is not None and t.shape != shape:
         raise ValueError("%s: %s must be %s, got %s" % (who, name, list(shape), list(t.shape)))
 
 
@@ -1154,7 +1167,11 @@ def _grad_slot(param):
 
 
 def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _workspace(n, like):
@@ -1166,24 +1183,22 @@ def embedding(idx, weight, scale=1.0, padding_idx=None):
     the rows sorted by token, in fp32 and in ascending row order: the same bits on every call, unlike EmbeddingFunction's
     atomics.  Rows equal to padding_idx give no gradient.  An id outside the table yields a NaN row and is reported by
     EmbeddingFunction.raise_if_bad()."""
-    _check_seq("embedding", weight)
-    if weight.dim() != 2:
-        raise ValueError("embedding: weight must be [tokens, dim], got %s" % (list(weight.shape),))
+    _check_input("embedding", weight, 2)
     if not torch.is_tensor(idx) or idx.dtype not in (torch.int64, torch.int32):
         raise TypeError("embedding: idx must be an int64 or int32 tensor")
-    if idx.device != weight.device:
+    if idx.get_device() != weight.get_device():
         raise RuntimeError("embedding: idx is on %s, the table on %s" % (idx.device, weight.device))
-    if weight.shape[1] < 1 or weight.shape[0] < 1:
+    vocab, pad = weight.shape[0], -1
+    if vocab < 1 or weight.shape[1] < 1:
         raise ValueError("embedding: empty table %s" % (list(weight.shape),))
-    pad = -1
     if padding_idx is not None:
         pad = int(padding_idx)
-        if not -weight.shape[0] <= pad < weight.shape[0]:
-            raise ValueError("embedding: padding_idx %d outside a table of %d" % (pad, weight.shape[0]))
-        pad %= weight.shape[0]
+        if not -vocab <= pad < vocab:
+            raise ValueError("embedding: padding_idx %d outside a table of %d" % (pad, vocab))
+        pad %= vocab
     _lib.require_gpu(weight)
     if _wants_grad(weight):
-        if idx.numel() >= 2 ** 31 or weight.shape[0] >= 2 ** 31 - 1:
+        if idx.numel() >= 2 ** 31 or vocab >= 2 ** 31 - 1:
             raise ValueError("embedding: the gradient takes fewer than 2^31 rows and tokens")
         return TokenEmbeddingFunction.apply(weight, idx, float(scale), pad)
     return _embedding_fwd(idx.to(torch.int64).contiguous(), weight, float(scale))
@@ -1199,10 +1214,10 @@ def _bad_flag(device):
 
 
 def _embedding_fwd(idx, weight, scale):
-    w = weight.detach().contiguous()
-    out = torch.empty(tuple(idx.shape) + (w.shape[1],), dtype=w.dtype, device=w.device)
-    _call_on(w, "jova_token_embedding_fwd", _ptr(w), _DTYPE_CODE[w.dtype], _ptr(idx), idx.numel(), w.shape[1], w.shape[0], scale,
-             _ptr(out), _ptr(_bad_flag(w.device)))
+    w, (v, d) = _c(weight), weight.shape
+    out = torch.empty((*idx.shape, d), dtype=w.dtype, device=w.device)
+    _call_on(w, "jova_token_embedding_fwd", w.data_ptr(), _DTYPE_CODE[w.dtype], idx.data_ptr(), idx.numel(), d, v, scale, out.data_ptr(),
+             _bad_flag(w.device).data_ptr())
     return out
 
 
@@ -1229,24 +1244,18 @@ class TokenEmbeddingFunction(torch.autograd.Function):
 
 
 def _conv_args(who, x, weight, bias, activation, dims):
-    if not torch.is_tensor(x) or x.dim() != dims:
-        raise ValueError("%s: x must have %d dimensions" % (who, dims))
-    _check_seq(who, x)
-    if weight.dim() != 2 or weight.shape[0] != x.shape[-1] or not 2 <= weight.shape[1] <= 8:
-        raise ValueError("%s: weight must be [%d, 2 .. 8], got %s" % (who, x.shape[-1], list(weight.shape)))
-    if x.shape[-1] < 1:
-        raise ValueError("%s: no channels" % who)
-    if weight.dtype not in (x.dtype, _F32):
+    _check_input(who, x, dims)
+    d = x.shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.dim() != 2 or weight.shape[0] != d or not 2 <= weight.shape[1] <= 8 or d < 1:
+        raise ValueError("%s: weight must be [%d, 2 .. 8], got %s" % (who, d, list(weight.shape) if torch.is_tensor(weight) else weight))
+    if weight.dtype != x.dtype and weight.dtype != _F32:
         raise TypeError("%s: weight must be %s or float32, got %s" % (who, x.dtype, weight.dtype))
-    _check_shape(who, "bias", bias, (weight.shape[0],))
-    for name, t in (("weight", weight), ("bias", bias)):
-        if t is not None and t.dtype != weight.dtype:
-            raise TypeError("%s: bias must have the weight's type" % who)
-        if t is not None and t.device != x.device:
-            raise RuntimeError("%s: %s is on %s, the input on %s" % (who, name, t.device, x.device))
-    if activation not in (None, "silu"):
+    _check_type(who, "weight", weight, weight.dtype, x)
+    _check_type(who, "bias", bias, weight.dtype, x)
+    _check_shape(who, "bias", bias, (d,))
+    if activation is not None and activation != "silu":
         raise ValueError("%s: activation must be None or 'silu', got %r" % (who, activation))
-    return int(activation == "silu")
+    return 0 if activation is None else 1
 
 
 def causal_conv1d(x, weight, bias=None, activation=None, lengths=None, initial_state=None, return_final_state=False):
@@ -1255,7 +1264,7 @@ def causal_conv1d(x, weight, bias=None, activation=None, lengths=None, initial_s
     holds the inputs in front of x (zeros without it).  Returns y, or (y, final_state) for the next piece of the sequence."""
     who = "causal_conv1d"
     silu = _conv_args(who, x, weight, bias, activation, 3)
-    _check_seq(who, x, initial_state=initial_state)
+    _check_type(who, "initial_state", initial_state, x.dtype, x)
     _check_shape(who, "initial_state", initial_state, (weight.shape[1] - 1, x.shape[1], x.shape[2]))
     lengths = _lengths_i32(who, lengths, x)
     _lib.require_gpu(x)
@@ -1267,8 +1276,7 @@ def causal_conv1d(x, weight, bias=None, activation=None, lengths=None, initial_s
 
 
 def _conv_fwd(x, weight, bias, state, lengths, silu, want_state):
-    x, w, b = _unit(x.detach()), _c(weight.detach()), None if bias is None else _c(bias.detach())
-    state = None if state is None else _c(state.detach())
+    x, w, b, state = _unit(x), _c(weight), _c_opt(bias), _c_opt(state)
     t, n, d = x.shape
     y = torch.empty((t, n, d), dtype=x.dtype, device=x.device)
     out = torch.empty((w.shape[1] - 1, n, d), dtype=x.dtype, device=x.device) if want_state else None
@@ -1289,10 +1297,10 @@ class CausalConvFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy, dstate_out):
         x, weight, bias, state, lengths = ctx.saved_tensors
-        x, w, b, state = _unit(x), _c(weight), None if bias is None else _c(bias), None if state is None else _c(state)
+        x, w, b, state = _unit(x), _c(weight), _c_opt(bias), _c_opt(state)
         t, n, d = x.shape
         dy = torch.zeros((t, n, d), dtype=x.dtype, device=x.device) if dy is None else _unit(dy)
-        dstate_out = None if dstate_out is None else _c(dstate_out)
+        dstate_out = _c_opt(dstate_out)
         dx = torch.empty((t, n, d), dtype=x.dtype, device=x.device)
         dstate = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
         # both parameter gradients in one way: accumulated in place only where both can be
@@ -1317,18 +1325,19 @@ class CausalConvFunction(torch.autograd.Function):
 
 def _out_state(who, state, out_state):
     """The tensor a single-token call writes the new state to: the old one (in place) or the caller's."""
-    if _wants_grad(state):
+    if state.requires_grad and torch.is_grad_enabled():
         raise RuntimeError("%s is for inference: the state requires grad" % who)
-    if out_state is None:
-        out_state = state
-    if out_state.shape != state.shape or out_state.dtype != state.dtype or out_state.device != state.device:
-        raise ValueError("%s: out_state must be like state" % who)
-    if not state.is_contiguous() or not out_state.is_contiguous():
+    if not state.is_contiguous():
         raise ValueError("%s: state and out_state must be contiguous" % who)
-    if out_state.data_ptr() != state.data_ptr():
-        lo, hi = sorted((state.data_ptr(), out_state.data_ptr()))
-        if state.numel() and hi < lo + state.numel() * state.element_size():
-            raise ValueError("%s: out_state overlaps state without being it" % who)
+    if out_state is None or out_state is state:
+        return state
+    _check_type(who, "out_state", out_state, state.dtype, state)
+    _check_shape(who, "out_state", out_state, state.shape)
+    if not out_state.is_contiguous():
+        raise ValueError("%s: state and out_state must be contiguous" % who)
+    a, b = state.data_ptr(), out_state.data_ptr()
+    if a != b and abs(a - b) < state.numel() * state.element_size():
+        raise ValueError("%s: out_state overlaps state without being it" % who)
     return out_state
 
 
@@ -1337,35 +1346,39 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, out_state=N
     The state moves on in place, or into out_state.  Inference only."""
     who = "causal_conv1d_step"
     silu = _conv_args(who, x, weight, bias, activation, 2)
-    _check_seq(who, x, state=state)
-    _check_shape(who, "state", state, (weight.shape[1] - 1,) + tuple(x.shape))
+    _check_type(who, "state", state, x.dtype, x)
+    _check_shape(who, "state", state, (weight.shape[1] - 1, *x.shape))
     if _wants_grad(x, weight, bias):
         raise RuntimeError("%s is for inference: run it under torch.no_grad()" % who)
     out = _out_state(who, state, out_state)
     _lib.require_gpu(x)
-    x, w, b = _unit(x), _c(weight), None if bias is None else _c(bias)
-    y = torch.empty(tuple(x.shape), dtype=x.dtype, device=x.device)
-    _call_on(x, "jova_causal_conv_step", _ptr(x), x.stride(0), _ptr(state), _ptr(out), _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1],
-             w.shape[1], _ptr(w), _ptr(b), _DTYPE_CODE[w.dtype], silu, _ptr(y))
+    x, w, (n, d) = _unit(x), _c(weight), x.shape
+    y = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    _call_on(x, "jova_causal_conv_step", x.data_ptr(), x.stride(0), state.data_ptr(), out.data_ptr(), _DTYPE_CODE[x.dtype], n, d,
+             w.shape[1], w.data_ptr(), _ptr(_c_opt(bias)), _DTYPE_CODE[w.dtype], silu, y.data_ptr())
     return y
 
 
-def _scan_check(who, x, dt, A, B, C, D, z, dt_bias):
-    _check_seq(who, x, dt=dt, B=B, C=C, z=z, A_f32=A, D_f32=D, dt_bias_f32=dt_bias)
-    lead, d = tuple(x.shape[:-1]), x.shape[-1]
+def _scan_check(who, x, dt, A, B, C, D, z, dt_bias, dims):
+    _check_input(who, x, dims)
+    kind, shape, d = x.dtype, x.shape, x.shape[-1]
+    for name, t in (("dt", dt), ("B", B), ("C", C), ("z", z)):
+        _check_type(who, name, t, kind, x)
+    for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
+        _check_type(who, name, t, _F32, x)
     if A.dim() != 2 or A.shape[0] != d or not 1 <= A.shape[1] <= 32:
         raise ValueError("%s: A must be [%d, 1 .. 32], got %s" % (who, d, list(A.shape)))
-    n = A.shape[1]
-    _check_shape(who, "dt", dt, x.shape)
-    _check_shape(who, "z", z, x.shape)
+    _check_shape(who, "dt", dt, shape)
+    _check_shape(who, "z", z, shape)
     _check_shape(who, "D", D, (d,))
     _check_shape(who, "dt_bias", dt_bias, (d,))
-    if B.shape != C.shape or tuple(B.shape[:len(lead)]) != lead or B.dim() not in (len(lead) + 1, len(lead) + 2) or B.shape[-1] != n:
-        raise ValueError("%s: B and C must be %s, got %s and %s" % (who, list(lead) + ["groups", n], list(B.shape), list(C.shape)))
-    if B.dim() == len(lead) + 1:
-        B, C = B.unsqueeze(-2), C.unsqueeze(-2)
-    if d < 1 or B.shape[-2] < 1 or d % B.shape[-2] != 0:
-        raise ValueError("%s: %d channels do not divide into %d groups" % (who, d, B.shape[-2]))
+    bs = B.shape
+    if bs != C.shape or len(bs) not in (dims, dims + 1) or bs[:dims - 1] != shape[:-1] or bs[-1] != A.shape[1]:
+        raise ValueError("%s: B and C must be %s, got %s and %s" % (who, list(shape[:-1]) + ["groups", A.shape[1]], list(bs), list(C.shape)))
+    if len(bs) == dims:
+        return B.unsqueeze(-2), C.unsqueeze(-2)
+    if d < 1 or bs[-2] < 1 or d % bs[-2] != 0:
+        raise ValueError("%s: %d channels do not divide into %d groups" % (who, d, bs[-2]))
     return B, C
 
 
@@ -1381,10 +1394,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
         e = dt + dt_bias (softplus of it with dt_softplus);  h[t] = exp(e A) h[t-1] + e x B;  y = (sum_n C h + D x) silu(z)
     Returns y, or (y, h behind the last step).  Differentiable in everything but lengths."""
     who = "selective_scan"
-    if not torch.is_tensor(x) or x.dim() != 3:
-        raise ValueError("%s: x must be [steps, batch, dim]" % who)
-    B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias)
-    _check_seq(who, x, initial_state_f32=initial_state)
+    B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias, 3)
+    _check_type(who, "initial_state", initial_state, _F32, x)
     _check_shape(who, "initial_state", initial_state, (x.shape[1], x.shape[2], A.shape[1]))
     lengths = _lengths_i32(who, lengths, x)
     _lib.require_gpu(x)
@@ -1396,13 +1407,12 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
 
 
 def _scan_dense(x, dt, A, B, C, D, z, dt_bias):
-    x, dt, z, B, C = (None if t is None else _unit(t.detach()) for t in (x, dt, z, B, C))
-    return (x, dt, _c(A.detach()), B, C, None if D is None else _c(D.detach()), z, None if dt_bias is None else _c(dt_bias.detach()))
+    return _unit(x), _unit(dt), _c(A), _unit(B), _unit(C), _c_opt(D), _unit(z), _c_opt(dt_bias)
 
 
 def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state, want_ckpt):
     x, dt, A, B, C, D, z, dt_bias = _scan_dense(x, dt, A, B, C, D, z, dt_bias)
-    state = None if state is None else _c(state.detach())
+    state = _c_opt(state)
     (t, b, d), n = x.shape, A.shape[1]
     y = torch.empty((t, b, d), dtype=x.dtype, device=x.device)
     h = torch.empty((b, d, n), dtype=_F32, device=x.device) if want_state else None
@@ -1430,7 +1440,7 @@ class SelectiveScanFunction(torch.autograd.Function):
         x, dt, A, B, C, D, z, dt_bias = _scan_dense(x, dt, A, B, C, D, z, dt_bias)
         (t, b, d), n, g = x.shape, A.shape[1], B.shape[2]
         dy = torch.zeros((t, b, d), dtype=x.dtype, device=x.device) if dy is None else _unit(dy)
-        dh = None if dh is None else _c(dh)
+        dh = _c_opt(dh)
         new = lambda *shape: torch.empty(shape, dtype=x.dtype, device=x.device)                 # noqa: E731
         new32 = lambda *shape: torch.empty(shape, dtype=_F32, device=x.device)                  # noqa: E731
         dx, ddt, dz = new(t, b, d), new(t, b, d), new(t, b, d) if z is not None else None
@@ -1449,21 +1459,20 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
     """One more step per sequence: x, dt, z [batch, dim], B, C [batch, groups, n] or [batch, n], state [batch, dim, n] float32
     (selective_scan's final state) -> y [batch, dim].  The state moves on in place, or into out_state.  Inference only."""
     who = "selective_scan_step"
-    if not torch.is_tensor(x) or x.dim() != 2:
-        raise ValueError("%s: x must be [batch, dim]" % who)
-    B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias)
-    _check_seq(who, x, state_f32=state)
-    _check_shape(who, "state", state, tuple(x.shape) + (A.shape[1],))
+    B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias, 2)
+    _check_type(who, "state", state, _F32, x)
+    _check_shape(who, "state", state, (*x.shape, A.shape[1]))
     if _wants_grad(x, dt, A, B, C, D, z, dt_bias):
         raise RuntimeError("%s is for inference: run it under torch.no_grad()" % who)
     out = _out_state(who, state, out_state)
     _lib.require_gpu(x)
     x, dt, A, B, C, D, z, dt_bias = _scan_dense(x, dt, A, B, C, D, z, dt_bias)
-    y = torch.empty(tuple(x.shape), dtype=x.dtype, device=x.device)
-    st = (ctypes.c_int64 * 12)(0, x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, B.stride(0), B.stride(1),
-                               0, C.stride(0), C.stride(1))
-    _call_on(x, "jova_selective_scan_step", _ptr(x), _ptr(dt), _ptr(A), _ptr(B), _ptr(C), _ptr(D), _ptr(z), _ptr(dt_bias),
-             _DTYPE_CODE[x.dtype], x.shape[0], x.shape[1], B.shape[1], A.shape[1], st, int(dt_softplus), _ptr(state), _ptr(out), _ptr(y))
+    b, d = x.shape
+    y = torch.empty((b, d), dtype=x.dtype, device=x.device)
+    st = (ctypes.c_int64 * 12)(0, x.stride(0), 0, dt.stride(0), 0, 0 if z is None else z.stride(0), 0, *B.stride()[:2], 0, *C.stride()[:2])
+    _call_on(x, "jova_selective_scan_step", x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(D), _ptr(z),
+             _ptr(dt_bias), _DTYPE_CODE[x.dtype], b, d, B.shape[1], A.shape[1], st, 1 if dt_softplus else 0, state.data_ptr(), out.data_ptr(),
+             y.data_ptr())
     return y
 
 

@@ -388,8 +388,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, norm_scale=1.0, out=Non
     """torch.nn.utils.clip_grad_norm_ on the HIP kernels: the norm over all gradients together, the gradients scaled in place
     by min(1, max_norm / (norm + 1e-6)); returns the norm as a float32 device scalar without reading it on the host.
 
-    ``parameters``: parameters (their ``.grad``; those without one are left out), plain tensors (themselves the gradients) or
-    a single one.  norm_type 2, 1 or inf.  norm_scale multiplies the norm only (1 / world size where the buffer holds the sum
+    ``parameters``: parameters or other tensors that require a gradient (their ``.grad``; those without one are left out), plain
+    tensors that do not (themselves the gradients), or a single one.  norm_type 2, 1 or inf.  norm_scale multiplies the norm only (1 / world size where the buffer holds the sum
     over the ranks and the optimizer divides).  ``out``: tensors that receive the clipped gradients, which then stay as
     they are.  A norm that is not finite makes the gradients so, as in torch."""
     kinds = {2.0: 2, 1.0: 1, float("inf"): 0}
@@ -399,7 +399,8 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, norm_scale=1.0, out=Non
     if not max_norm >= 0.0:
         raise ValueError("clip_grad_norm_: max_norm must not be negative, got %r" % max_norm)
     params = [parameters] if torch.is_tensor(parameters) else list(parameters)
-    grads = [p.grad if isinstance(p, nn.Parameter) or (p.requires_grad and p.is_leaf) else p for p in params]
+    # (isinstance(.., nn.Parameter) costs more than all other checks together: asked only of what might be a frozen one)
+    grads = [p.grad if p.requires_grad or (type(p) is not torch.Tensor and isinstance(p, nn.Parameter)) else p for p in params]
     grads = [g for g in grads if g is not None]
     if out is not None:
         out = [out] if torch.is_tensor(out) else list(out)
