@@ -9,6 +9,8 @@
 
 namespace {
 
+constexpr int FWD_BYTES = 8, BWD_BYTES = 8;           // of one thread's channels
+
 struct ConvArgs {
     const void *x, *dy, *weight, *bias, *state, *dstate_out;
     void *y, *dx, *state_out, *dstate;
@@ -25,117 +27,188 @@ __device__ __forceinline__ long long seq_len(const ConvArgs& a, int b) {
     return n < 0 ? 0 : n > a.steps ? a.steps : n;
 }
 
-// x[t] of channel c for t in [-(W-1), len)
-template <typename T, int W>
-__device__ __forceinline__ float conv_in(const ConvArgs& a, long long t, int b, int c, long long len) {
-    if (t >= len) return 0.f;
-    if (t >= 0) return to_f(((const T*)a.x)[t * a.x_t + b * a.x_b + c]);
-    return a.state ? to_f(((const T*)a.state)[((t + W - 1) * a.batch + b) * (long long)a.d + c]) : 0.f;
+// V neighbouring channels of one step
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+template <typename T, int V> __device__ __forceinline__ Pack<T, V> none() {
+    Pack<T, V> p;
+#pragma unroll
+    for (int i = 0; i < V; ++i) p.v[i] = from_f<T>(0.f);
+    return p;
+}
+// x[t] for t in [-(W-1), len), zero elsewhere
+template <typename T, int W, int V>
+__device__ __forceinline__ Pack<T, V> conv_in(const ConvArgs& a, long long t, int b, int c, long long len) {
+    if (t >= len) return none<T, V>();
+    if (t >= 0) return *(const Pack<T, V>*)((const T*)a.x + t * a.x_t + b * a.x_b + c);
+    return a.state ? *(const Pack<T, V>*)((const T*)a.state + ((t + W - 1) * a.batch + b) * (long long)a.d + c) : none<T, V>();
 }
 
-template <typename T, int W>
+// A thread owns V channels (16 bytes where the rows allow it: conv_vec) of a.chunk steps and keeps the window in registers;
+// U steps are loaded before the first of them is used.
+template <typename T, int W, int V>
 __global__ void __launch_bounds__(256)
 conv_fwd_kernel(ConvArgs a) {
-    const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+    constexpr int U = 16;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * V, b = blockIdx.y;
     if (c >= a.d) return;
     const long long len = seq_len(a, b), t0 = (long long)blockIdx.z * a.chunk, t1 = min(a.steps, t0 + a.chunk);
-    float w[W], win[W];
+    float w[V][W], bias[V], win[W][V];
 #pragma unroll
-    for (int k = 0; k < W; ++k) w[k] = ld_any(a.weight, a.wtype, (long long)c * W + k);
-    const float bias = a.bias ? ld_any(a.bias, a.wtype, c) : 0.f;
+    for (int v = 0; v < V; ++v) {
+        bias[v] = a.bias ? ld_any(a.bias, a.wtype, c + v) : 0.f;
 #pragma unroll
-    for (int k = 0; k + 1 < W; ++k) win[k + 1] = conv_in<T, W>(a, t0 - W + 1 + k, b, c, len);
-    T* y = (T*)a.y;
-    for (long long t = t0; t < t1; ++t) {
-#pragma unroll
-        for (int k = 0; k + 1 < W; ++k) win[k] = win[k + 1];
-        win[W - 1] = conv_in<T, W>(a, t, b, c, len);
-        float p = bias;
-#pragma unroll
-        for (int k = 0; k < W; ++k) p = fmaf(w[k], win[k], p);
-        if (a.silu) p *= sigmoid_f(p);
-        y[(t * a.batch + b) * (long long)a.d + c] = from_f<T>(t < len ? p : 0.f);
+        for (int k = 0; k < W; ++k) w[v][k] = ld_any(a.weight, a.wtype, (long long)(c + v) * W + k);
     }
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k) {
+        const Pack<T, V> p = conv_in<T, W, V>(a, t0 - W + 1 + k, b, c, len);
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[k + 1][v] = to_f(p.v[v]);
+    }
+    T* y = (T*)a.y + b * (long long)a.d + c;
+    const long long y_t = (long long)a.batch * a.d;
+    auto one = [&](const Pack<T, V>& in, long long t, bool live) {
+        Pack<T, V> out;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+#pragma unroll
+            for (int k = 0; k + 1 < W; ++k) win[k][v] = win[k + 1][v];
+            win[W - 1][v] = to_f(in.v[v]);
+            float p = bias[v];
+#pragma unroll
+            for (int k = 0; k < W; ++k) p = fmaf(w[v][k], win[k][v], p);
+            if (a.silu) p *= sigmoid_f(p);
+            out.v[v] = from_f<T>(live ? p : 0.f);
+        }
+        *(Pack<T, V>*)(y + t * y_t) = out;
+    };
+    long long t = t0;
+    for (; t + U <= min(t1, len); t += U) {
+        const T* x = (const T*)a.x + t * a.x_t + b * a.x_b + c;
+        Pack<T, V> in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) in[u] = *(const Pack<T, V>*)(x + u * a.x_t);
+#pragma unroll
+        for (int u = 0; u < U; ++u) one(in[u], t + u, true);
+    }
+    for (; t < t1; ++t) one(conv_in<T, W, V>(a, t, b, c, len), t, t < len);
     if (a.state_out && blockIdx.z == 0) {
-        T* so = (T*)a.state_out;
 #pragma unroll
         for (int k = 0; k + 1 < W; ++k)
-            so[((long long)k * a.batch + b) * a.d + c] = from_f<T>(conv_in<T, W>(a, len - W + 1 + k, b, c, len));
+            *(Pack<T, V>*)((T*)a.state_out + ((long long)k * a.batch + b) * a.d + c) = conv_in<T, W, V>(a, len - W + 1 + k, b, c, len);
     }
 }
 
-template <typename T, int W>
+template <typename T, int W, int V>
 __global__ void __launch_bounds__(256)
 conv_bwd_kernel(ConvArgs a) {
-    const int c = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+    constexpr int U = 8;
+    const int c = (blockIdx.x * 256 + threadIdx.x) * V, b = blockIdx.y;
     if (c >= a.d) return;
     const long long len = seq_len(a, b), t0 = (long long)blockIdx.z * a.chunk, t1 = min(a.steps, t0 + a.chunk);
-    float w[W], win[W], acc[W], dw[W], db = 0.f;
+    float w[V][W], bias[V], win[W][V], acc[W][V], dw[W][V], db[V];
 #pragma unroll
-    for (int k = 0; k < W; ++k) {
-        w[k] = ld_any(a.weight, a.wtype, (long long)c * W + k);
-        dw[k] = 0.f;
-        acc[k] = 0.f;                                  // acc[j] = dx[t - W + 1 + j], complete in j = 0 after step t
+    for (int v = 0; v < V; ++v) {
+        bias[v] = a.bias ? ld_any(a.bias, a.wtype, c + v) : 0.f;
+        db[v] = 0.f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            w[v][k] = ld_any(a.weight, a.wtype, (long long)(c + v) * W + k);
+            dw[k][v] = 0.f;
+            acc[k][v] = 0.f;                           // acc[j] = dx[t - W + 1 + j], complete in j = 0 after step t
+        }
     }
-    const float bias = a.bias ? ld_any(a.bias, a.wtype, c) : 0.f;
 #pragma unroll
-    for (int k = 0; k + 1 < W; ++k) win[k + 1] = conv_in<T, W>(a, t0 - W + 1 + k, b, c, len);
-    T* dx = (T*)a.dx;
+    for (int k = 0; k + 1 < W; ++k) {
+        const Pack<T, V> p = conv_in<T, W, V>(a, t0 - W + 1 + k, b, c, len);
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[k + 1][v] = to_f(p.v[v]);
+    }
+    T* dx = (T*)a.dx + b * (long long)a.d + c;
+    const long long dx_t = (long long)a.batch * a.d;
     const T *dy = (const T*)a.dy, *dso = (const T*)a.dstate_out;
     const long long lo = (a.dstate && blockIdx.z == 0) ? -(W - 1) : t0;        // chunk 0 also owns the initial state
-    for (long long t = t0; t < t1 + W - 1; ++t) {
+    // step t: x[t] and dy[t] in (zeros behind the end: they add nothing), dx[t - W + 1] out; own: the step's terms of dw and dbias count
+    auto one = [&](const Pack<T, V>& in, const Pack<T, V>& g, long long t, bool own, bool inner) {
+        Pack<T, V> out;
+        const long long s = t - W + 1, j = s - (len - (W - 1));
+        Pack<T, V> so = none<T, V>();                  // gradient of the returned state, which holds x[len - W + 1 .. len)
+        if (!inner && dso && j >= 0 && s < len) so = *(const Pack<T, V>*)(dso + (j * a.batch + b) * a.d + c);
 #pragma unroll
-        for (int k = 0; k + 1 < W; ++k) {
-            win[k] = win[k + 1];
-            acc[k] = acc[k + 1];
-        }
-        acc[W - 1] = 0.f;
-        win[W - 1] = conv_in<T, W>(a, t, b, c, len);
-        if (t < len) {
-            float p = bias;
+        for (int v = 0; v < V; ++v) {
 #pragma unroll
-            for (int k = 0; k < W; ++k) p = fmaf(w[k], win[k], p);
-            float dp = to_f(dy[t * a.dy_t + b * a.dy_b + c]);
+            for (int k = 0; k + 1 < W; ++k) {
+                win[k][v] = win[k + 1][v];
+                acc[k][v] = acc[k + 1][v];
+            }
+            win[W - 1][v] = to_f(in.v[v]);
+            float dp = to_f(g.v[v]);
             if (a.silu) {
-                const float s = sigmoid_f(p);
-                dp *= s * (1.f + p * (1.f - s));
-            }
-            if (t < t1) db += dp;
+                float p = bias[v];
 #pragma unroll
-            for (int k = 0; k < W; ++k) {
-                acc[k] = fmaf(w[k], dp, acc[k]);
-                if (t < t1) dw[k] = fmaf(dp, win[k], dw[k]);
+                for (int k = 0; k < W; ++k) p = fmaf(w[v][k], win[k][v], p);
+                const float sg = sigmoid_f(p);
+                dp *= sg * (1.f + p * (1.f - sg));
             }
+            if (!inner && t >= len) dp = 0.f;
+            acc[W - 1][v] = 0.f;
+#pragma unroll
+            for (int k = 0; k < W; ++k) acc[k][v] = fmaf(w[v][k], dp, acc[k][v]);
+            if (own) {
+                db[v] += dp;
+#pragma unroll
+                for (int k = 0; k < W; ++k) dw[k][v] = fmaf(dp, win[k][v], dw[k][v]);
+            }
+            out.v[v] = from_f<T>(acc[0][v] + to_f(so.v[v]));
         }
-        const long long s = t - W + 1;
         if (s >= lo && s < t1) {
-            float v = acc[0];
-            const long long j = s - (len - (W - 1));   // its place in the state that the forward returned
-            if (dso && j >= 0 && s < len) v += to_f(dso[(j * a.batch + b) * a.d + c]);
-            if (s >= 0) dx[(s * a.batch + b) * (long long)a.d + c] = from_f<T>(s < len ? v : 0.f);
-            else ((T*)a.dstate)[((s + W - 1) * a.batch + b) * (long long)a.d + c] = from_f<T>(v);
+            if (s >= 0) *(Pack<T, V>*)(dx + s * dx_t) = (inner || s < len) ? out : none<T, V>();
+            else *(Pack<T, V>*)((T*)a.dstate + ((s + W - 1) * a.batch + b) * (long long)a.d + c) = out;
         }
+    };
+    long long t = t0;
+    for (; t + U <= min(t1, len); t += U) {
+        // the last W - 1 inputs in front of the end take the gradient of the returned state too
+        const bool inner = !dso || t + U <= len - (W - 1);
+        const T *x = (const T*)a.x + t * a.x_t + b * a.x_b + c, *g = dy + t * a.dy_t + b * a.dy_b + c;
+        Pack<T, V> in[U], gr[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            in[u] = *(const Pack<T, V>*)(x + u * a.x_t);
+            gr[u] = *(const Pack<T, V>*)(g + u * a.dy_t);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) one(in[u], gr[u], t + u, true, inner);
     }
+    for (; t < t1 + W - 1; ++t)
+        one(conv_in<T, W, V>(a, t, b, c, len), t < len ? *(const Pack<T, V>*)(dy + t * a.dy_t + b * a.dy_b + c) : none<T, V>(), t, t < t1, false);
     float* part = a.part + ((long long)blockIdx.z * a.batch + b) * (W + 1) * a.d + c;
 #pragma unroll
-    for (int k = 0; k < W; ++k) part[(long long)k * a.d] = dw[k];
-    part[(long long)W * a.d] = db;
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) part[(long long)k * a.d + v] = dw[k][v];
+        part[(long long)W * a.d + v] = db[v];
+    }
 }
 
-// dw[c][k], dbias[c] from the partial sums, rows in order
-__global__ void __launch_bounds__(256)
+// dw[c][k], dbias[c] from the partial sums: 16 waves take every 16th row of 64 channels, then wave order
+__global__ void __launch_bounds__(1024)
 conv_fold_kernel(const float* __restrict__ part, long long rows, int d, int width, void* __restrict__ dw, void* __restrict__ db,
                  int wtype, int accumulate) {
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = blockIdx.y, g = threadIdx.x >> 6;
-    __shared__ double red[4][64];
+    const int l = threadIdx.x & 63, g = threadIdx.x >> 6, c = blockIdx.x * 64 + l, k = blockIdx.y;
+    __shared__ double red[16][64];
     double s = 0.0;
-    if (c < d)
-        for (long long r = g; r < rows; r += 4) s += (double)part[(r * (width + 1) + k) * d + c];
-    red[g][threadIdx.x & 63] = s;
+    if (c < d) {
+        const float* p = part + (long long)k * d + c;
+        const long long row = (long long)(width + 1) * d;
+#pragma unroll 8
+        for (long long r = g; r < rows; r += 16) s += (double)p[r * row];
+    }
+    red[g][l] = s;
     __syncthreads();
     if (g != 0 || c >= d) return;
-    const int l = threadIdx.x;
-    float v = (float)((red[0][l] + red[1][l]) + (red[2][l] + red[3][l]));
+    for (int i = 1; i < 16; ++i) s += red[i][l];
+    float v = (float)s;
     void* to = k < width ? dw : db;
     if (!to) return;
     const long long at = k < width ? (long long)c * width + k : c;
@@ -164,7 +237,17 @@ conv_step_kernel(const T* x, long long x_b, const T* state, T* state_out, const 
 
 int conv_chunk(int64_t steps) { return 64; }
 
-// calls f.template operator()<T, W>()
+// channels a thread takes: as many as fit `bytes` and divide the rows, the strides and the addresses of all tensors
+int conv_vec(int dtype, int bytes, const ConvArgs& a) {
+    const int es = (int)jova_dtype_size(dtype);
+    int v = bytes / es;
+    const uintptr_t at = (uintptr_t)a.x | (uintptr_t)a.dy | (uintptr_t)a.y | (uintptr_t)a.dx | (uintptr_t)a.state | (uintptr_t)a.state_out |
+                         (uintptr_t)a.dstate | (uintptr_t)a.dstate_out;
+    const long long st = a.x_t | a.x_b | a.dy_t | a.dy_b | a.d;
+    return (st % v == 0 && at % (uintptr_t)(v * es) == 0) ? v : 1;
+}
+
+// calls f(T(), width constant)
 template <typename F> int conv_dispatch(int dtype, int width, F f) {
 #define JOVA_CONV_W(W)                                                     \
     case W:                                                                \
@@ -206,9 +289,13 @@ extern "C" int jova_causal_conv_fwd(const void* x, int64_t x_t, int64_t x_b, int
     a.x = x; a.weight = weight; a.bias = bias_or_null; a.state = state_or_null; a.y = y; a.state_out = state_out_or_null;
     a.lengths = lengths_or_null; a.x_t = x_t; a.x_b = x_b; a.steps = steps; a.batch = (int)batch; a.d = d; a.silu = silu;
     a.wtype = weight_dtype; a.chunk = conv_chunk(steps);
-    const dim3 grid((d + 255) / 256, (unsigned)batch, (unsigned)(steps ? (steps + a.chunk - 1) / a.chunk : 1));
+    const int v = conv_vec(dtype, FWD_BYTES, a), per = 256 * v;
+    const dim3 grid((d + per - 1) / per, (unsigned)batch, (unsigned)(steps ? (steps + a.chunk - 1) / a.chunk : 1));
     return conv_dispatch(dtype, width, [&](auto t, auto w) {
-        hipLaunchKernelGGL((conv_fwd_kernel<decltype(t), decltype(w)::value>), grid, dim3(256), 0, (hipStream_t)stream, a);
+        typedef decltype(t) T;
+        constexpr int W = decltype(w)::value;
+        if (v > 1) hipLaunchKernelGGL((conv_fwd_kernel<T, W, FWD_BYTES / sizeof(T)>), grid, dim3(256), 0, (hipStream_t)stream, a);
+        else hipLaunchKernelGGL((conv_fwd_kernel<T, W, 1>), grid, dim3(256), 0, (hipStream_t)stream, a);
         JOVA_CHECK_LAUNCH("causal_conv_fwd");
         return JOVA_OK;
     });
@@ -234,15 +321,19 @@ extern "C" int jova_causal_conv_bwd(const void* x, int64_t x_t, int64_t x_b, con
     const long long chunks = (steps + a.chunk - 1) / a.chunk;
     const hipStream_t s = (hipStream_t)stream;
     if (steps > 0 && batch > 0) {
-        const dim3 grid((d + 255) / 256, (unsigned)batch, (unsigned)chunks);
+        const int v = conv_vec(dtype, BWD_BYTES, a), per = 256 * v;
+        const dim3 grid((d + per - 1) / per, (unsigned)batch, (unsigned)chunks);
         const int rc = conv_dispatch(dtype, width, [&](auto t, auto w) {
-            hipLaunchKernelGGL((conv_bwd_kernel<decltype(t), decltype(w)::value>), grid, dim3(256), 0, s, a);
+            typedef decltype(t) T;
+            constexpr int W = decltype(w)::value;
+            if (v > 1) hipLaunchKernelGGL((conv_bwd_kernel<T, W, BWD_BYTES / sizeof(T)>), grid, dim3(256), 0, s, a);
+            else hipLaunchKernelGGL((conv_bwd_kernel<T, W, 1>), grid, dim3(256), 0, s, a);
             JOVA_CHECK_LAUNCH("causal_conv_bwd");
             return JOVA_OK;
         });
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(conv_fold_kernel, dim3((d + 63) / 64, width + (dbias_or_null ? 1 : 0)), dim3(256), 0, s, a.part,
+    hipLaunchKernelGGL(conv_fold_kernel, dim3((d + 63) / 64, width + (dbias_or_null ? 1 : 0)), dim3(1024), 0, s, a.part,
                        (long long)(steps > 0 ? chunks * batch : 0), d, width, dweight, dbias_or_null, weight_dtype, accumulate);
     JOVA_CHECK_LAUNCH("causal_conv_bwd (fold)");
     return JOVA_OK;

@@ -8,12 +8,10 @@
 
 namespace {
 
-constexpr int SORT_THREADS = 256;
-constexpr int SORT_WAVES = SORT_THREADS / 64;
-constexpr int SORT_ROUND = 2048;                       // items a workgroup ranks at a time: 8 x 64 per wave
-constexpr int SORT_ITERS = SORT_ROUND / SORT_THREADS;
-constexpr int SORT_MAX_BLOCKS = 1024;                  // beyond: longer spans per workgroup (the count table stays small)
-constexpr int RADIX = 256;
+constexpr int SORT_THREADS = 512, SORT_WAVES = SORT_THREADS / 64;
+constexpr int SORT_ITERS = 4, SORT_ROUND = SORT_THREADS * SORT_ITERS;          // items a workgroup ranks at a time
+constexpr int SORT_MAX_BLOCKS = 128;                    // beyond: longer spans per workgroup; every one reads all counts
+constexpr int MAX_BITS = 9, RADIX = 1 << MAX_BITS;     // of a pass: 18-bit tokens in two passes, 14-bit ones too (7 + 7)
 
 struct SortPlan {
     int bits, passes, digit_bits, blocks;
@@ -23,141 +21,233 @@ SortPlan sort_plan(long long n, long long vocab) {
     SortPlan p;
     p.bits = 1;
     while ((1ll << p.bits) < vocab + 1) ++p.bits;      // vocab itself = "no gradient", sorts behind every token
-    p.passes = (p.bits + 7) / 8;
+    p.passes = (p.bits + MAX_BITS - 1) / MAX_BITS;
     p.digit_bits = (p.bits + p.passes - 1) / p.passes;
-    p.span = SORT_ROUND;
-    while ((n + p.span - 1) / p.span > SORT_MAX_BLOCKS) p.span += SORT_ROUND;
+    p.span = ((n + SORT_MAX_BLOCKS - 1) / SORT_MAX_BLOCKS + SORT_ROUND - 1) / SORT_ROUND * SORT_ROUND;
     p.blocks = (int)((n + p.span - 1) / p.span);
     return p;
 }
 
-__device__ __forceinline__ unsigned token_key(const long long* idx, long long r, long long vocab, long long pad) {
-    const long long k = idx[r];
-    return (k < 0 || k >= vocab || k == pad) ? (unsigned)vocab : (unsigned)k;
+struct SortArgs {
+    const long long* idx;                              // first pass: the tokens
+    const uint2* in;                                   // later passes: (token, row)
+    uint2* out;
+    unsigned* counts;                                  // [block][1 << digit_bits]
+    long long n, vocab, pad, span;
+    int shift, digit_bits;
+    // workgroups behind the sort's own fill this launch's share of dW with zeros: a sort keeps at most 128 of 256 CUs busy
+    int blocks;
+    uint4* zero;
+    long long z0, z1;
+    unsigned char* rest;                               // the last bytes of dW that are no 16
+    int n_rest;
+};
+__device__ __forceinline__ bool zero_share(const SortArgs& a) {
+    if ((int)blockIdx.x < a.blocks) return false;
+    const long long step = (long long)(gridDim.x - a.blocks) * SORT_THREADS;
+    for (long long i = a.z0 + (long long)((int)blockIdx.x - a.blocks) * SORT_THREADS + threadIdx.x; i < a.z1; i += step)
+        a.zero[i] = make_uint4(0u, 0u, 0u, 0u);
+    if ((int)blockIdx.x == a.blocks && (int)threadIdx.x < a.n_rest) a.rest[threadIdx.x] = 0;
+    return true;
+}
+__device__ __forceinline__ uint2 sort_item(const SortArgs& a, long long i) {
+    if (!a.idx) return a.in[i];
+    const long long k = a.idx[i];
+    return make_uint2((k < 0 || k >= a.vocab || k == a.pad) ? (unsigned)a.vocab : (unsigned)k, (unsigned)i);
 }
 
-// counts[digit][block] of this pass's digit.  Integer LDS atomics: the counts do not depend on their order.
+// counts of this pass's digit.  Integer LDS atomics: the counts do not depend on their order.
 __global__ void __launch_bounds__(SORT_THREADS)
-token_hist_kernel(const long long* __restrict__ idx, const uint2* __restrict__ in, long long n, long long vocab, long long pad,
-                  int shift, int mask, long long span, unsigned* __restrict__ counts) {
+token_hist_kernel(SortArgs a) {
     __shared__ unsigned cnt[RADIX];
-    for (int i = threadIdx.x; i <= mask; i += SORT_THREADS) cnt[i] = 0;
+    if (zero_share(a)) return;
+    const int radix = 1 << a.digit_bits;
+    if ((int)threadIdx.x < radix) cnt[threadIdx.x] = 0;
     __syncthreads();
-    const long long lo = blockIdx.x * span, hi = min(n, lo + span);
-    for (long long i = lo + threadIdx.x; i < hi; i += SORT_THREADS) {
-        const unsigned k = idx ? token_key(idx, i, vocab, pad) : in[i].x;
-        atomicAdd(&cnt[(k >> shift) & mask], 1u);
-    }
+    const long long lo = blockIdx.x * a.span, hi = min(a.n, lo + a.span);
+#pragma unroll 4
+    for (long long i = lo + threadIdx.x; i < hi; i += SORT_THREADS) atomicAdd(&cnt[(sort_item(a, i).x >> a.shift) & (radix - 1)], 1u);
     __syncthreads();
-    for (int i = threadIdx.x; i <= mask; i += SORT_THREADS) counts[(long long)i * gridDim.x + blockIdx.x] = cnt[i];
+    if ((int)threadIdx.x < radix) a.counts[blockIdx.x * radix + threadIdx.x] = cnt[threadIdx.x];
 }
 
-// exclusive prefix sum of m counts in place, one workgroup
-__global__ void __launch_bounds__(1024)
-token_scan_kernel(unsigned* __restrict__ counts, int m) {
-    __shared__ unsigned wsum[16];
-    __shared__ unsigned carry;
+// exclusive prefix sum over the workgroup's threads
+__device__ __forceinline__ unsigned block_prefix(unsigned v, unsigned* wsum) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    if (threadIdx.x == 0) carry = 0;
-    __syncthreads();
-    for (int base = 0; base < m; base += 1024) {
-        const int i = base + threadIdx.x;
-        const unsigned v = i < m ? counts[i] : 0;
-        unsigned s = v;
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned u = __shfl_up(s, o, 64);
-            if (lane >= o) s += u;
-        }
-        if (lane == 63) wsum[w] = s;
-        __syncthreads();
-        unsigned before = carry;
-        for (int k = 0; k < w; ++k) before += wsum[k];
-        if (i < m) counts[i] = before + s - v;
-        __syncthreads();
-        if (threadIdx.x == 1023) carry = before + s;
-        __syncthreads();
+    unsigned s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned u = __shfl_up(s, o, 64);
+        if (lane >= o) s += u;
     }
+    if (lane == 63) wsum[w] = s;
+    __syncthreads();
+    unsigned before = 0;
+    for (int k = 0; k < w; ++k) before += wsum[k];
+    __syncthreads();
+    return before + s - v;
 }
 
-// Stable scatter by this pass's digit.  Every wave owns consecutive items of the round; equal digits of 64 items find each
-// other by one ballot per digit bit, so an item's rank is (earlier ones of its wave) + (peers in lower lanes), without atomics.
+// LDS accesses of a wave's lanes on either side stay on theirs (the hardware keeps a wave's LDS operations in order)
+__device__ __forceinline__ void wave_order() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Ranks one round of items: every wave owns consecutive ones; equal digits of 64 items find each other by one ballot per digit
+// bit, so an item's rank is (earlier ones of its wave) + (peers in lower lanes), without atomics.  Leaves each wave's counts.
+__device__ __forceinline__ void rank_round(const SortArgs& a, long long r0, long long hi, unsigned (*wcnt)[RADIX], uint2* item, unsigned* rank) {
+    const int radix = 1 << a.digit_bits, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int i = lane; i < radix; i += 64) wcnt[w][i] = 0;
+#pragma unroll
+    for (int it = 0; it < SORT_ITERS; ++it) {
+        const long long i = r0 + (w * SORT_ITERS + it) * 64 + lane;
+        item[it] = i < hi ? sort_item(a, i) : make_uint2(0, 0);
+    }
+    wave_order();
+#pragma unroll
+    for (int it = 0; it < SORT_ITERS; ++it) {
+        const bool live = r0 + (w * SORT_ITERS + it) * 64 + lane < hi;
+        const unsigned dg = (item[it].x >> a.shift) & (radix - 1);
+        unsigned long long peers = __ballot(live);
+        for (int b = 0; b < a.digit_bits; ++b) {
+            const unsigned long long bal = __ballot((dg >> b) & 1u);
+            peers &= ((dg >> b) & 1u) ? bal : ~bal;
+        }
+        const int below = __popcll(peers & ((1ull << lane) - 1ull));
+        unsigned before = 0;
+        if (live) before = wcnt[w][dg];
+        wave_order();                                  // every lane has read its count
+        if (live && below == 0) wcnt[w][dg] = before + (unsigned)__popcll(peers);
+        wave_order();
+        rank[it] = before + below;
+    }
+}
+__device__ __forceinline__ void place_round(const SortArgs& a, long long r0, long long hi, const unsigned (*wcnt)[RADIX], const uint2* item,
+                                            const unsigned* rank) {
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+#pragma unroll
+    for (int it = 0; it < SORT_ITERS; ++it)
+        if (r0 + (w * SORT_ITERS + it) * 64 + lane < hi)
+            a.out[wcnt[w][(item[it].x >> a.shift) & ((1 << a.digit_bits) - 1)] + rank[it]] = item[it];
+}
+
+// Stable scatter by this pass's digit; the places come from all workgroups' counts, read by each (at most 128 x 512)
 __global__ void __launch_bounds__(SORT_THREADS)
-token_scatter_kernel(const long long* __restrict__ idx, const uint2* __restrict__ in, long long n, long long vocab, long long pad,
-                     int shift, int digit_bits, long long span, const unsigned* __restrict__ counts, uint2* __restrict__ out) {
+token_scatter_kernel(SortArgs a) {
     __shared__ unsigned wcnt[SORT_WAVES][RADIX];
-    __shared__ unsigned base[RADIX];
-    const int radix = 1 << digit_bits, mask = radix - 1;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    for (int i = threadIdx.x; i < radix; i += SORT_THREADS) base[i] = counts[(long long)i * gridDim.x + blockIdx.x];
-    const long long lo = blockIdx.x * span, hi = min(n, lo + span);
+    __shared__ unsigned base[RADIX], total[RADIX], wsum[SORT_WAVES];
+    if (zero_share(a)) return;
+    const int radix = 1 << a.digit_bits, me = blockIdx.x, blocks = a.blocks;
+    const int dg = threadIdx.x & (radix - 1), part = threadIdx.x >> a.digit_bits, parts = SORT_THREADS >> a.digit_bits;
+    if ((int)threadIdx.x < radix) base[threadIdx.x] = total[threadIdx.x] = 0;
+    __syncthreads();
+    unsigned before = 0, all = 0;
+#pragma unroll 8
+    for (int k = part; k < blocks; k += parts) {
+        const unsigned c = a.counts[k * radix + dg];
+        all += c;
+        before += k < me ? c : 0;
+    }
+    if (parts == 1) {
+        base[dg] = before;
+        total[dg] = all;
+    } else {
+        atomicAdd(&base[dg], before);                  // (integers)
+        atomicAdd(&total[dg], all);
+    }
+    __syncthreads();
+    const unsigned pre = block_prefix((int)threadIdx.x < radix ? total[threadIdx.x] : 0, wsum);
+    if ((int)threadIdx.x < radix) base[threadIdx.x] += pre;
+    const long long lo = me * a.span, hi = min(a.n, lo + a.span);
+    uint2 item[SORT_ITERS];
+    unsigned rank[SORT_ITERS];
     for (long long r0 = lo; r0 < hi; r0 += SORT_ROUND) {
-        for (int i = lane; i < radix; i += 64) wcnt[w][i] = 0;
-        uint2 item[SORT_ITERS];
-        unsigned rank[SORT_ITERS];
-#pragma unroll
-        for (int it = 0; it < SORT_ITERS; ++it) {
-            const long long i = r0 + w * (SORT_ROUND / SORT_WAVES) + it * 64 + lane;
-            item[it] = i >= hi ? make_uint2(0, 0) : idx ? make_uint2(token_key(idx, i, vocab, pad), (unsigned)i) : in[i];
-        }
-        __syncthreads();                               // the round before has read wcnt and base
-#pragma unroll
-        for (int it = 0; it < SORT_ITERS; ++it) {
-            const bool live = r0 + w * (SORT_ROUND / SORT_WAVES) + it * 64 + lane < hi;
-            const unsigned dg = (item[it].x >> shift) & mask;
-            unsigned long long peers = __ballot(live);
-            for (int b = 0; b < digit_bits; ++b) {
-                const unsigned long long bal = __ballot((dg >> b) & 1u);
-                peers &= ((dg >> b) & 1u) ? bal : ~bal;
-            }
-            const int below = __popcll(peers & ((1ull << lane) - 1ull));
-            unsigned before = 0;
-            if (live) before = wcnt[w][dg];
-            __builtin_amdgcn_wave_barrier();           // every lane has read its count (LDS is in order within a wave)
-            if (live && below == 0) wcnt[w][dg] = before + (unsigned)__popcll(peers);
-            __builtin_amdgcn_wave_barrier();
-            rank[it] = before + below;
-        }
+        rank_round(a, r0, hi, wcnt, item, rank);
         __syncthreads();
-        for (int i = threadIdx.x; i < radix; i += SORT_THREADS) {      // counts -> first places, wave by wave
-            unsigned at = base[i];
+        if ((int)threadIdx.x < radix) {                // counts -> first places, wave by wave
+            unsigned at = base[threadIdx.x];
+#pragma unroll
             for (int k = 0; k < SORT_WAVES; ++k) {
-                const unsigned c = wcnt[k][i];
-                wcnt[k][i] = at;
+                const unsigned c = wcnt[k][threadIdx.x];
+                wcnt[k][threadIdx.x] = at;
                 at += c;
             }
-            base[i] = at;
+            base[threadIdx.x] = at;
         }
         __syncthreads();
-#pragma unroll
-        for (int it = 0; it < SORT_ITERS; ++it)
-            if (r0 + w * (SORT_ROUND / SORT_WAVES) + it * 64 + lane < hi)
-                out[wcnt[w][(item[it].x >> shift) & mask] + rank[it]] = item[it];
+        place_round(a, r0, hi, wcnt, item, rank);
         __syncthreads();
+    }
+}
+
+// All passes of a sort that one round holds, in one workgroup and one launch
+__global__ void __launch_bounds__(SORT_THREADS)
+token_sort_small_kernel(SortArgs a, int passes, uint2* buf0, uint2* buf1) {
+    __shared__ unsigned wcnt[SORT_WAVES][RADIX];
+    __shared__ unsigned wsum[SORT_WAVES];
+    if (zero_share(a)) return;
+    const int radix = 1 << a.digit_bits;
+    uint2 item[SORT_ITERS];
+    unsigned rank[SORT_ITERS];
+    for (int p = 0; p < passes; ++p) {
+        a.shift = p * a.digit_bits;
+        a.out = p & 1 ? buf1 : buf0;
+        rank_round(a, 0, a.n, wcnt, item, rank);
+        __syncthreads();
+        unsigned all = 0;
+        if ((int)threadIdx.x < radix)
+#pragma unroll
+            for (int k = 0; k < SORT_WAVES; ++k) all += wcnt[k][threadIdx.x];
+        unsigned at = block_prefix(all, wsum);
+        if ((int)threadIdx.x < radix)
+#pragma unroll
+            for (int k = 0; k < SORT_WAVES; ++k) {
+                const unsigned c = wcnt[k][threadIdx.x];
+                wcnt[k][threadIdx.x] = at;
+                at += c;
+            }
+        __syncthreads();
+        place_round(a, 0, a.n, wcnt, item, rank);
+        __threadfence_block();
+        __syncthreads();
+        a.idx = nullptr;
+        a.in = a.out;
     }
 }
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
 
-template <typename T, int VEC>
+// I: the index type that holds n * dv (64-bit divisions cost more than the row's copy)
+template <typename T, int VEC, typename I>
 __global__ void __launch_bounds__(256)
 token_fwd_kernel(const T* __restrict__ w, const long long* __restrict__ idx, long long n, int dv, long long vocab, float scale,
                  T* __restrict__ out, int* __restrict__ bad) {
-    const long long total = n * dv;
-    for (long long e = (long long)blockIdx.x * blockDim.x + threadIdx.x; e < total; e += (long long)gridDim.x * blockDim.x) {
-        const long long r = e / dv;
-        const int c = (int)(e - r * dv);
-        const long long k = idx[r];
-        Pack<T, VEC> p;
-        if (k < 0 || k >= vocab) {                     // nn.Embedding raises: flag it, emit NaN
-            if (c == 0) atomicOr(bad, 1);
+    constexpr int U = 4;                               // rows requested before the first of them is written
+    const I total = (I)(n * dv), step = (I)gridDim.x * 256;
+    for (I e0 = (I)blockIdx.x * 256 + threadIdx.x; e0 < total; e0 += U * step) {
+        Pack<T, VEC> p[U];
+        bool ok[U];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) p.v[j] = from_f<T>(__int_as_float(0x7fc00000));
-        } else {
-            p = reinterpret_cast<const Pack<T, VEC>*>(w)[k * dv + c];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) p.v[j] = from_f<T>(to_f(p.v[j]) * scale);
+        for (int u = 0; u < U; ++u) {
+            const I e = e0 + u * step;
+            ok[u] = false;
+            if (e >= total) continue;
+            const I r = e / (I)dv;
+            const int c = (int)(e - r * (I)dv);
+            const long long k = idx[r];
+            ok[u] = k >= 0 && k < vocab;
+            if (ok[u]) p[u] = reinterpret_cast<const Pack<T, VEC>*>(w)[k * dv + c];
+            else if (c == 0) atomicOr(bad, 1);         // nn.Embedding raises: flag it, emit NaN
         }
-        reinterpret_cast<Pack<T, VEC>*>(out)[e] = p;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const I e = e0 + u * step;
+            if (e >= total) continue;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) p[u].v[j] = from_f<T>(ok[u] ? to_f(p[u].v[j]) * scale : __int_as_float(0x7fc00000));
+            reinterpret_cast<Pack<T, VEC>*>(out)[e] = p[u];
+        }
     }
 }
 
@@ -173,66 +263,118 @@ __device__ __forceinline__ void write_row(T* dw, long long at, const float* acc,
     reinterpret_cast<Pack<T, VEC>*>(dw)[at] = p;
 }
 
+constexpr int TILE = 32;                               // entries of a tile
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256)
-token_reduce_kernel(const uint2* __restrict__ order, const T* __restrict__ dout, long long n, int dv, unsigned vocab, int tile,
-                    int gw, float scale, int accumulate, T* __restrict__ dw, float* __restrict__ head, float* __restrict__ tail) {
-    const int per = 256 / gw;
-    const long long t = (long long)blockIdx.x * per + threadIdx.x / gw;
+token_reduce_kernel(const uint2* __restrict__ order, const T* __restrict__ dout, long long n, int dv, unsigned vocab, int gw, float scale,
+                    int accumulate, T* __restrict__ dw, float* __restrict__ head, float* __restrict__ tail) {
+    constexpr int U = 8;                               // rows requested before the first of them is added
+    const int per = 256 / gw, g = threadIdx.x / gw;
+    const long long t = (long long)blockIdx.x * per + g, e0 = t * TILE;
     const int c = blockIdx.y * 256 + threadIdx.x % gw;
-    const long long e0 = t * tile;
+    __shared__ uint2 lds[32][TILE + 2];                // a tile's entries between its neighbours' (at most 256 / 8 tiles)
+    for (int i = threadIdx.x % gw; i < TILE + 2; i += gw) {
+        const long long e = e0 - 1 + i;
+        lds[g][i] = e >= 0 && e < n ? order[e] : make_uint2(~0u, 0);
+    }
+    __syncthreads();
     if (e0 >= n || c >= dv) return;
-    const long long e1 = min(n, e0 + tile);
-    const unsigned prev = e0 > 0 ? order[e0 - 1].x : ~0u, next = e1 < n ? order[e1].x : ~0u;
+    const uint2* it = lds[g] + 1;
+    const Pack<T, VEC>* rows = reinterpret_cast<const Pack<T, VEC>*>(dout) + c;
     float acc[VEC];
-    unsigned cur = order[e0].x;
-    bool open = cur == prev;                           // the run began in an earlier tile
+    unsigned cur = it[0].x;
+    bool open = cur == it[-1].x;                       // the run began in an earlier tile
 #pragma unroll
     for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-    for (long long e = e0; e <= e1; ++e) {
-        const uint2 it = e < e1 ? order[e] : make_uint2(~0u, 0);
-        if (it.x != cur) {
-            if (cur != vocab) {
-                float* part = open ? head : (e == e1 && cur == next) ? tail : nullptr;
-                if (part) {
+    Pack<T, VEC> p[U], ahead[U];
 #pragma unroll
-                    for (int j = 0; j < VEC; ++j) part[(t * dv + c) * VEC + j] = acc[j];
-                } else {
-                    write_row<T, VEC>(dw, (long long)cur * dv + c, acc, scale, accumulate);
+    for (int u = 0; u < U; ++u)
+        if (it[u].x < vocab) ahead[u] = rows[(long long)it[u].y * dv];
+    for (int e = 0; e < TILE; e += U) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) p[u] = ahead[u];
+        if (e + U < TILE)                              // in front of this batch's stores: a load behind a store waits for it
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (it[e + U + u].x < vocab) ahead[u] = rows[(long long)it[e + U + u].y * dv];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const unsigned key = it[e + u].x;
+            if (key != cur) {                          // the run ends inside the tile
+                if (cur < vocab) {
+                    if (open) {
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) head[(t * dv + c) * VEC + j] = acc[j];
+                    } else {
+                        write_row<T, VEC>(dw, (long long)cur * dv + c, acc, scale, accumulate);
+                    }
                 }
+                cur = key;
+                open = false;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
             }
-            if (e == e1) return;
-            cur = it.x;
-            open = false;
+            if (key < vocab)                           // (vocab: no gradient; ~0: behind the last entry)
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+                for (int j = 0; j < VEC; ++j) acc[j] += to_f(p[u].v[j]);
         }
-        if (cur == vocab) return;                      // sorted behind every token: nothing follows
-        const Pack<T, VEC> p = reinterpret_cast<const Pack<T, VEC>*>(dout)[(long long)it.y * dv + c];
+    }
+    if (cur >= vocab) return;
+    float* part = open ? head : it[TILE].x == cur ? tail : nullptr;
+    if (part) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += to_f(p.v[j]);
+        for (int j = 0; j < VEC; ++j) part[(t * dv + c) * VEC + j] = acc[j];
+    } else {
+        write_row<T, VEC>(dw, (long long)cur * dv + c, acc, scale, accumulate);
     }
 }
 
+// The runs that cross a border: the tile a run begins in adds its tail and the heads of the tiles behind it, `parts` groups of lanes
+// every parts-th tile each, then group by group.  A run's end is found by doubling and bisection over the tiles' first entries:
+// most runs end in the next tile, a hot token's has thousands.
 template <typename T, int VEC>
-__global__ void __launch_bounds__(256)
-token_join_kernel(const uint2* __restrict__ order, long long n, int dv, unsigned vocab, int tile, int gw, float scale,
-                  int accumulate, T* __restrict__ dw, const float* __restrict__ head, const float* __restrict__ tail) {
-    const int per = 256 / gw;
-    const long long t = (long long)blockIdx.x * per + threadIdx.x / gw;
-    const int c = blockIdx.y * 256 + threadIdx.x % gw;
-    const long long e0 = t * tile, e1 = e0 + tile;
-    if (e1 >= n || c >= dv) return;                    // the last tile has no run that goes on
+__global__ void __launch_bounds__(1024)
+token_join_kernel(const uint2* __restrict__ order, long long n, int dv, unsigned vocab, int gw, int parts, float scale, int accumulate,
+                  T* __restrict__ dw, const float* __restrict__ head, const float* __restrict__ tail) {
+    __shared__ float red[1024 * VEC];
+    const int g = threadIdx.x / gw, c = blockIdx.y * 256 + threadIdx.x % gw;
+    const long long t = blockIdx.x, e0 = t * TILE, e1 = e0 + TILE;       // (all conditions are the workgroup's)
+    if (e1 >= n) return;                               // the last tile has no run that goes on
     const unsigned key = order[e1 - 1].x;
-    if (key == vocab || order[e1].x != key) return;
-    if (order[e0].x == key && e0 > 0 && order[e0 - 1].x == key) return;      // began earlier: that tile joins it
+    if (key >= vocab || order[e1].x != key) return;
+    if (e0 > 0 && order[e0 - 1].x == key) return;      // began earlier: that tile joins it
+    const long long tiles = (n + TILE - 1) / TILE;
+    long long last = t + 1, hi = t + 2;                // last: begins with the key; hi: does not (once found)
+    for (long long by = 1; hi < tiles && order[hi * TILE].x == key; by *= 2) {
+        last = hi;
+        hi = last + 2 * by;
+    }
+    hi = min(hi, tiles);
+    while (hi - last > 1) {
+        const long long mid = (last + hi) >> 1;
+        if (order[mid * TILE].x == key) last = mid; else hi = mid;
+    }
     float acc[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) acc[j] = tail[(t * dv + c) * VEC + j];
-    for (long long u = t + 1; u * tile < n && order[u * tile].x == key; ++u) {
+    for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
+    if (c < dv) {
+        if (g == 0) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) acc[j] += head[(u * dv + c) * VEC + j];
+            for (int j = 0; j < VEC; ++j) acc[j] = tail[(t * dv + c) * VEC + j];
+        }
+#pragma unroll 4
+        for (long long u = t + 1 + g; u <= last; u += parts) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) acc[j] += head[(u * dv + c) * VEC + j];
+        }
     }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) red[j * 1024 + threadIdx.x] = acc[j];
+    __syncthreads();
+    if (g != 0 || c >= dv) return;
+    for (int k = 1; k < parts; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) acc[j] += red[j * 1024 + k * gw + threadIdx.x];
     write_row<T, VEC>(dw, (long long)key * dv + c, acc, scale, accumulate);
 }
 
@@ -242,9 +384,6 @@ __global__ void token_zero_kernel(unsigned char* __restrict__ p, long long n16, 
     if (blockIdx.x == 0 && (int)threadIdx.x < rest) p[n16 * 16 + threadIdx.x] = 0;
 }
 
-constexpr int REDUCE_TILE = 32;
-int reduce_tile(long long n) { return REDUCE_TILE; }
-
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 int vec_of(int d, size_t esz, const void* a, const void* b) {
@@ -253,12 +392,21 @@ int vec_of(int d, size_t esz, const void* a, const void* b) {
     return vec;
 }
 
+int gw_of(int dv) {
+    int gw = 8;
+    while (gw < 256 && gw < dv) gw <<= 1;
+    return gw;
+}
+
 template <typename T, int VEC>
 int fwd_launch(const void* w, const int64_t* idx, int64_t n, int d, int64_t vocab, float scale, void* out, int* bad, hipStream_t s) {
-    const long long total = n * (d / VEC);
-    const int blocks = (int)(total + 255 < 256ll * 8192 ? (total + 255) / 256 : 8192);
-    hipLaunchKernelGGL((token_fwd_kernel<T, VEC>), dim3(blocks), dim3(256), 0, s, (const T*)w, (const long long*)idx, (long long)n,
-                       d / VEC, (long long)vocab, scale, (T*)out, bad);
+    const int dv = d / VEC;
+    const long long total = n * dv, want = (total + 255) / 256;
+    const dim3 grid((unsigned)(want < 8192 ? want : 8192));
+    if (total < (1ll << 31)) hipLaunchKernelGGL((token_fwd_kernel<T, VEC, unsigned>), grid, dim3(256), 0, s, (const T*)w, (const long long*)idx,
+                                                (long long)n, dv, (long long)vocab, scale, (T*)out, bad);
+    else hipLaunchKernelGGL((token_fwd_kernel<T, VEC, unsigned long long>), grid, dim3(256), 0, s, (const T*)w, (const long long*)idx,
+                            (long long)n, dv, (long long)vocab, scale, (T*)out, bad);
     JOVA_CHECK_LAUNCH("token_embedding_fwd");
     return JOVA_OK;
 }
@@ -275,17 +423,16 @@ int fwd_dispatch(const void* w, const int64_t* idx, int64_t n, int d, int64_t vo
 template <typename T, int VEC>
 int reduce_launch(const uint2* order, const void* dout, int64_t n, int d, int64_t vocab, float scale, int accumulate, void* dw,
                   float* head, float* tail, hipStream_t s) {
-    const int dv = d / VEC, tile = reduce_tile(n);
-    int gw = 8;
-    while (gw < 256 && gw < dv) gw <<= 1;
-    const long long tiles = (n + tile - 1) / tile;
-    const dim3 grid((unsigned)((tiles + 256 / gw - 1) / (256 / gw)), (unsigned)((dv + 255) / 256));
-    hipLaunchKernelGGL((token_reduce_kernel<T, VEC>), grid, dim3(256), 0, s, order, (const T*)dout, (long long)n, dv, (unsigned)vocab,
-                       tile, gw, scale, accumulate, (T*)dw, head, tail);
+    const int dv = d / VEC, gw = gw_of(dv), per = 256 / gw;
+    const long long tiles = (n + TILE - 1) / TILE;
+    const unsigned cols = (unsigned)((dv + 255) / 256);
+    hipLaunchKernelGGL((token_reduce_kernel<T, VEC>), dim3((unsigned)((tiles + per - 1) / per), cols), dim3(256), 0, s, order, (const T*)dout,
+                       (long long)n, dv, (unsigned)vocab, gw, scale, accumulate, (T*)dw, head, tail);
     JOVA_CHECK_LAUNCH("token_embedding_bwd (reduce)");
     if (tiles > 1) {
-        hipLaunchKernelGGL((token_join_kernel<T, VEC>), grid, dim3(256), 0, s, order, (long long)n, dv, (unsigned)vocab, tile, gw, scale,
-                           accumulate, (T*)dw, head, tail);
+        const int threads = gw <= 64 ? 256 : 4 * gw;
+        hipLaunchKernelGGL((token_join_kernel<T, VEC>), dim3((unsigned)(tiles - 1), cols), dim3(threads), 0, s, order, (long long)n, dv,
+                           (unsigned)vocab, gw, threads / gw, scale, accumulate, (T*)dw, head, tail);
         JOVA_CHECK_LAUNCH("token_embedding_bwd (join)");
     }
     return JOVA_OK;
@@ -316,7 +463,7 @@ extern "C" int jova_token_embedding_fwd(const void* weight, int dtype, const int
 extern "C" size_t jova_token_embedding_bwd_workspace_bytes(int64_t n, int d, int64_t vocab) {
     if (n <= 0 || d < 1 || vocab < 1) return 256;
     const SortPlan p = sort_plan(n, vocab);
-    const size_t tiles = (size_t)((n + reduce_tile(n) - 1) / reduce_tile(n));
+    const size_t tiles = (size_t)((n + TILE - 1) / TILE);
     return 2 * align256((size_t)n * 8) + align256((size_t)RADIX * p.blocks * 4) + 2 * align256(tiles * d * 4);
 }
 
@@ -327,12 +474,18 @@ extern "C" int jova_token_embedding_bwd(const void* dout, int dtype, const int64
     JOVA_CHECK_ARG(n >= 0 && d >= 1 && vocab >= 1 && dweight && (n == 0 || (dout && idx && workspace)), "token_embedding_bwd: bad argument");
     JOVA_CHECK_ARG(n < (1ll << 31) && vocab < (1ll << 31) - 1, "token_embedding_bwd: at most 2^31 - 1 rows and tokens");
     hipStream_t s = (hipStream_t)stream;
+    long long n16 = 0;
+    int n_rest = 0;
     if (!accumulate) {
         const long long bytes = (long long)vocab * d * (long long)jova_dtype_size(dtype);
         JOVA_CHECK_ARG((((uintptr_t)dweight) & 15) == 0, "token_embedding_bwd: dweight must start on a 16-byte boundary");
-        const int blocks = (int)(bytes / 16 / 256 + 1 < 8192 ? bytes / 16 / 256 + 1 : 8192);
-        hipLaunchKernelGGL(token_zero_kernel, dim3(blocks), dim3(256), 0, s, (unsigned char*)dweight, bytes / 16, (int)(bytes & 15));
-        JOVA_CHECK_LAUNCH("token_embedding_bwd (zero)");
+        n16 = bytes / 16;
+        n_rest = (int)(bytes & 15);
+        if (n == 0) {
+            const int blocks = (int)(n16 / 256 + 1 < 8192 ? n16 / 256 + 1 : 8192);
+            hipLaunchKernelGGL(token_zero_kernel, dim3(blocks), dim3(256), 0, s, (unsigned char*)dweight, n16, n_rest);
+            JOVA_CHECK_LAUNCH("token_embedding_bwd (zero)");
+        }
     }
     if (n == 0) return JOVA_OK;
     const SortPlan p = sort_plan(n, vocab);
@@ -341,21 +494,41 @@ extern "C" int jova_token_embedding_bwd(const void* dout, int dtype, const int64
     ws += 2 * align256((size_t)n * 8);
     unsigned* counts = (unsigned*)ws;
     ws += align256((size_t)RADIX * p.blocks * 4);
-    const int tile = reduce_tile(n);
-    const size_t tiles = (size_t)((n + tile - 1) / tile);
+    const size_t tiles = (size_t)((n + TILE - 1) / TILE);
     float* head = (float*)ws;
     float* tail = (float*)(ws + align256(tiles * d * 4));
-    const int mask = (1 << p.digit_bits) - 1;
-    const uint2* in = nullptr;
-    for (int k = 0; k < p.passes; ++k) {
-        const long long* first = k == 0 ? (const long long*)idx : nullptr;
-        hipLaunchKernelGGL(token_hist_kernel, dim3(p.blocks), dim3(SORT_THREADS), 0, s, first, in, (long long)n, (long long)vocab,
-                           (long long)padding_idx, k * p.digit_bits, mask, p.span, counts);
-        hipLaunchKernelGGL(token_scan_kernel, dim3(1), dim3(1024), 0, s, counts, (mask + 1) * p.blocks);
-        hipLaunchKernelGGL(token_scatter_kernel, dim3(p.blocks), dim3(SORT_THREADS), 0, s, first, in, (long long)n, (long long)vocab,
-                           (long long)padding_idx, k * p.digit_bits, p.digit_bits, p.span, counts, buf[k & 1]);
+    SortArgs a = {};
+    a.idx = (const long long*)idx; a.counts = counts; a.n = n; a.vocab = vocab; a.pad = padding_idx; a.span = p.span;
+    a.digit_bits = p.digit_bits; a.blocks = p.blocks; a.zero = (uint4*)dweight;
+    const bool small = n <= SORT_ROUND;
+    const int launches = small ? 1 : 2 * p.passes;
+    int done = 0;
+    // (the k-th launch's share of the zeros, and the grid that it takes: 16 x 16 bytes a lane at least)
+    auto grid = [&]() {
+        a.z0 = n16 * done / launches;
+        a.z1 = n16 * (done + 1) / launches;
+        a.n_rest = ++done == launches ? n_rest : 0;
+        a.rest = (unsigned char*)dweight + n16 * 16;
+        const long long zb = (a.z1 - a.z0 + 16 * SORT_THREADS - 1) / (16 * SORT_THREADS);
+        return dim3((unsigned)(p.blocks + (zb < 1024 ? zb : 1024) + (zb == 0 && a.n_rest ? 1 : 0)));
+    };
+    const uint2* in = buf[(p.passes - 1) & 1];
+    if (small) {
+        const dim3 small_grid = grid();
+        hipLaunchKernelGGL(token_sort_small_kernel, small_grid, dim3(SORT_THREADS), 0, s, a, p.passes, buf[0], buf[1]);
         JOVA_CHECK_LAUNCH("token_embedding_bwd (sort)");
-        in = buf[k & 1];
+    } else {
+        for (int k = 0; k < p.passes; ++k) {
+            a.shift = k * p.digit_bits;
+            a.out = buf[k & 1];
+            const dim3 hist_grid = grid();
+            hipLaunchKernelGGL(token_hist_kernel, hist_grid, dim3(SORT_THREADS), 0, s, a);
+            const dim3 scatter_grid = grid();
+            hipLaunchKernelGGL(token_scatter_kernel, scatter_grid, dim3(SORT_THREADS), 0, s, a);
+            JOVA_CHECK_LAUNCH("token_embedding_bwd (sort)");
+            a.idx = nullptr;
+            a.in = a.out;
+        }
     }
     if (dtype == JOVA_F32) return reduce_dispatch<float>(in, dout, n, d, vocab, scale, accumulate, dweight, head, tail, s);
     if (dtype == JOVA_BF16) return reduce_dispatch<bf16_t>(in, dout, n, d, vocab, scale, accumulate, dweight, head, tail, s);
