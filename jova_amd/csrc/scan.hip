@@ -69,54 +69,83 @@ __device__ __forceinline__ Where where(const ScanArgs& a) {
     return w;
 }
 
-// One value per lane: element (t, b, channel) of a [steps, batch, d] tensor.  The part of the address that is the same for the
-// wave stays in scalar registers (base of step t0, advanced by scalar arithmetic), the lane's own part is a 32-bit offset
-// that never changes: strides are checked on the host (LANE_LIMIT).
+// One value per lane: element (t, b, channel) of a [steps, batch, d] tensor, t = tile + 4 j + q.  What is the same for the wave
+// stays in scalar registers and moves on with the tiles; the lane's own part is a 32-bit offset that never changes (strides
+// are checked on the host: lane_ok).
 template <typename T> struct Lane {
-    const char* base;                                  // of batch element b
-    long long step;                                    // bytes
-    unsigned off;                                      // q * step + channel, bytes
-    __device__ __forceinline__ Lane() {}
-    __device__ __forceinline__ Lane(const void* p, long long s_t, long long s_b, const Where& w)
-        : base((const char*)p + w.b * s_b * (long long)sizeof(T)), step(s_t * (long long)sizeof(T)),
+    const char* at;                                    // of the tile, batch element b
+    long long step4;                                   // bytes of four steps
+    unsigned off;                                      // (q * step + channel), bytes
+    __device__ __forceinline__ Lane(const void* p, long long s_t, long long s_b, const Where& w, long long t0)
+        : at((const char*)p + (t0 * s_t + w.b * s_b) * (long long)sizeof(T)), step4(4 * s_t * (long long)sizeof(T)),
           off((unsigned)(w.q * s_t + w.ch) * (unsigned)sizeof(T)) {}
-    __device__ __forceinline__ T load(long long t0) const { return *(const T*)(base + t0 * step + off); }
-    __device__ __forceinline__ void store(long long t0, float v) const { *(T*)(const_cast<char*>(base) + t0 * step + off) = from_f<T>(v); }
-};
-// KT / 4 steps of one tensor, as stored; steps behind the end are not touched
-template <typename T, int J> struct Steps {
-    T v[J];
-    __device__ __forceinline__ void load(const Lane<T>& l, bool there, long long t0, long long len, int q) {
-        if (!there) return;
-        if (t0 + 4 * J <= len) {
+    __device__ __forceinline__ T load(int j) const { return *(const T*)(at + j * step4 + off); }
+    __device__ __forceinline__ void store(int j, float v) const { *(T*)(const_cast<char*>(at) + j * step4 + off) = from_f<T>(v); }
+    __device__ __forceinline__ void move(int tiles_j) { at += tiles_j * step4; }
+    // values of a tile's steps, those before `rem` (of the sequence) as computed, the others (of the tensor) as zeros
+    template <int J> __device__ __forceinline__ void store_tile(const float* v, int rem, int there, int q) const {
+        if (rem >= 4 * J) {
 #pragma unroll
-            for (int j = 0; j < J; ++j) v[j] = l.load(t0 + 4 * j);
+            for (int j = 0; j < J; ++j) store(j, v[j]);
         } else {
 #pragma unroll
-            for (int j = 0; j < J; ++j) v[j] = t0 + 4 * j + q < len ? l.load(t0 + 4 * j) : from_f<T>(0.f);
+            for (int j = 0; j < J; ++j)
+                if (4 * j + q < there) store(j, 4 * j + q < rem ? v[j] : 0.f);
+        }
+    }
+};
+// steps of a tile that are left of `len`
+template <int KT> __device__ __forceinline__ int left_of(long long len, long long t0) {
+    const long long r = len - t0;
+    return r >= KT ? KT : r < 0 ? 0 : (int)r;
+}
+// a tile's values as stored; steps behind the end are not touched
+template <typename T, int J> struct Steps {
+    T v[J];
+    __device__ __forceinline__ void load(const Lane<T>& l, int rem, int q) {
+        if (rem >= 4 * J) {
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[j] = l.load(j);
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[j] = 4 * j + q < rem ? l.load(j) : from_f<T>(0.f);
         }
     }
 };
 
-// rows of B and C of KT steps -> LDS, fp32, zero behind the sequence and in the padded states
+// a tile's rows of B and C -> LDS, fp32, zero behind the sequence and in the padded states
 template <typename T, int NS>
 struct Rows {
     static constexpr int KT = Tile<NS>::KT, NP = 4 * NS, PER = (2 * KT * NP + 255) / 256;
     T v[PER];
-    __device__ __forceinline__ void load(const ScanArgs& a, const Where& w, long long t0) {
+    const char* at[PER];
+    long long tile[PER];                               // bytes of a tile
+    int t[PER];                                        // step within the tile; KT: nothing to load
+    __device__ __forceinline__ Rows(const ScanArgs& a, const Where& w, long long t0, bool with_B) {
 #pragma unroll
         for (int r = 0; r < PER; ++r) {
-            const int i = threadIdx.x + 256 * r, n = i % NP, t = (i / NP) % KT;
-            v[r] = from_f<T>(0.f);
-            if (i >= 2 * KT * NP || n >= a.n || t0 + t >= w.len) continue;
-            v[r] = i < KT * NP ? ((const T*)a.B)[(t0 + t) * a.B_t + w.b * a.B_b + w.g * a.B_g + n]
-                               : ((const T*)a.C)[(t0 + t) * a.C_t + w.b * a.C_b + w.g * a.C_g + n];
+            const int i = threadIdx.x + 256 * r, n = i % NP;
+            const bool isB = i < KT * NP;
+            t[r] = (i / NP) % KT;
+            const long long s_t = isB ? a.B_t : a.C_t;
+            at[r] = (const char*)(isB ? a.B : a.C) +
+                    ((t0 + t[r]) * s_t + w.b * (isB ? a.B_b : a.C_b) + w.g * (isB ? a.B_g : a.C_g) + n) * (long long)sizeof(T);
+            tile[r] = KT * s_t * (long long)sizeof(T);
+            if (i >= 2 * KT * NP || n >= a.n || (isB && !with_B)) t[r] = KT;
         }
+    }
+    __device__ __forceinline__ void load(int rem) {
+#pragma unroll
+        for (int r = 0; r < PER; ++r) v[r] = t[r] < rem ? *(const T*)at[r] : from_f<T>(0.f);
+    }
+    __device__ __forceinline__ void move(int tiles) {
+#pragma unroll
+        for (int r = 0; r < PER; ++r) at[r] += tiles * tile[r];
     }
     __device__ __forceinline__ void put(float* lds) const {
 #pragma unroll
         for (int r = 0; r < PER; ++r)
-            if (threadIdx.x + 256 * r < 2 * KT * NP) lds[threadIdx.x + 256 * r] = to_f(v[r]);
+            if (PER * 256 == 2 * KT * NP || threadIdx.x + 256 * r < 2 * KT * NP) lds[threadIdx.x + 256 * r] = to_f(v[r]);
     }
 };
 
@@ -169,6 +198,9 @@ template <typename F> __device__ __forceinline__ void four_back(F f) {
     f(std::integral_constant<int, 0>());
 }
 
+// The loops below have no branch between a tile's loads and its stores: options (softplus, the gate) are selects, without z its
+// loads read x.
+
 // LOCAL: the chunk's own contribution to the state (from zero) and its sum of e, for carry_in
 template <typename T, int NS, bool LOCAL>
 __global__ void __launch_bounds__(256)
@@ -176,7 +208,7 @@ scan_fwd_kernel(ScanArgs a) {
     constexpr int KT = Tile<NS>::KT, NP = 4 * NS, J = KT / 4;
     __shared__ __align__(16) float rows[2][2 * KT * NP];
     const Where w = where(a);
-    const bool b0 = w.q & 1, b1 = w.q & 2;
+    const bool b0 = w.q & 1, b1 = w.q & 2, softplus = a.softplus, gate = a.z != nullptr;
     const long long first = (long long)blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk);
     float A2[NS], h[NS], es = 0.f;
     load_A2<NS>(a, w, A2);
@@ -188,36 +220,40 @@ scan_fwd_kernel(ScanArgs a) {
         carry_in<NS>(a, w, A2, 0, blockIdx.z, 1, h);
     }
     const float Dv = a.D ? a.D[w.ch] : 0.f, bias = a.bias ? a.bias[w.ch] : 0.f;
-    const Lane<T> lx(a.x, a.x_t, a.x_b, w), ldt(a.dt, a.dt_t, a.dt_b, w), lz(a.z, a.z_t, a.z_b, w),
-        ly(a.y, (long long)a.batch * a.d, a.d, w);
-    Rows<T, NS> rn;
+    Lane<T> lx(a.x, a.x_t, a.x_b, w, first), ldt(a.dt, a.dt_t, a.dt_b, w, first);
+    Lane<T> lz(gate ? a.z : a.x, gate ? a.z_t : a.x_t, gate ? a.z_b : a.x_b, w, first), ly(a.y, (long long)a.batch * a.d, a.d, w, first);
+    Rows<T, NS> rn(a, w, first, true);
     Steps<T, J> xn, dn, zn;
-    auto fetch = [&](long long t0) {
-        rn.load(a, w, t0);
-        xn.load(lx, true, t0, w.len, w.q);
-        dn.load(ldt, true, t0, w.len, w.q);
-        if (!LOCAL) zn.load(lz, a.z != nullptr, t0, w.len, w.q);
+    int rem = left_of<KT>(w.len, first);
+    auto fetch = [&]() {
+        rn.load(rem);
+        xn.load(lx, rem, w.q);
+        dn.load(ldt, rem, w.q);
+        if (!LOCAL) zn.load(lz, rem, w.q);
     };
-    fetch(first);
+    fetch();
     rn.put(rows[0]);
     __syncthreads();
     int cur = 0;
     for (long long t0 = first; t0 < last; t0 += KT, cur ^= 1) {
-        float x[J], e[J], z[J];
-        const bool full = t0 + KT <= w.len;
+        float x[J], e[J], z[J], y[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             x[j] = to_f(xn.v[j]);
-            const float raw = to_f(dn.v[j]) + bias;
-            e[j] = a.softplus ? softplus_f(raw) : raw;
+            const float raw = to_f(dn.v[j]) + bias, sp = softplus_f(raw);
+            e[j] = 4 * j + w.q < rem ? (softplus ? sp : raw) : 0.f;
             if (!LOCAL) z[j] = to_f(zn.v[j]);
         }
-        if (!full) {
-#pragma unroll
-            for (int j = 0; j < J; ++j)
-                if (t0 + 4 * j + w.q >= w.len) e[j] = 0.f;
+        const int now = rem;
+        const bool more = t0 + KT < last;
+        if (more) {
+            rn.move(1);
+            lx.move(J);
+            ldt.move(J);
+            lz.move(J);
+            rem = left_of<KT>(w.len, t0 + KT);
+            fetch();
         }
-        if (t0 + KT < last) fetch(t0 + KT);
         if (!LOCAL && a.ckpt && w.live) {
             Part<NS> p;
 #pragma unroll
@@ -242,13 +278,15 @@ scan_fwd_kernel(ScanArgs a) {
                 }
             });
             if (!LOCAL) {
-                float y = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
-                if (a.z) y *= z[j] * sigmoid_f(z[j]);
-                const long long t = t0 + 4 * j + w.q;
-                if (w.live && (full || t < a.steps)) ly.store(t0 + 4 * j, full || t < w.len ? y : 0.f);
+                const float v = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
+                y[j] = gate ? v * (z[j] * sigmoid_f(z[j])) : v;
             }
         }
-        if (t0 + KT < last) rn.put(rows[cur ^ 1]);
+        if (!LOCAL) {
+            if (w.live) ly.template store_tile<J>(y, now, left_of<KT>(a.steps, t0), w.q);
+            ly.move(J);
+        }
+        if (more) rn.put(rows[cur ^ 1]);
         __syncthreads();
     }
     if (LOCAL) {
@@ -269,45 +307,61 @@ template <typename T, int NS>
 __global__ void __launch_bounds__(256)
 scan_adjoint_kernel(ScanArgs a) {
     constexpr int KT = Tile<NS>::KT, NP = 4 * NS, J = KT / 4;
-    __shared__ __align__(16) float rows[2 * KT * NP];
+    __shared__ __align__(16) float rows[2][2 * KT * NP];
     const Where w = where(a);
+    const bool softplus = a.softplus, gate = a.z != nullptr;
     const int chunk = blockIdx.z + 1;                  // nothing is in front of chunk 0
-    const long long first = (long long)chunk * a.chunk, last = min(a.steps, first + a.chunk);
+    const long long first = (long long)chunk * a.chunk, last = min(a.steps, first + a.chunk), top = first + ((last - first - 1) / KT) * KT;
     float A2[NS], q[NS], es = 0.f;
     load_A2<NS>(a, w, A2);
 #pragma unroll
     for (int k = 0; k < NS; ++k) q[k] = 0.f;
     const float bias = a.bias ? a.bias[w.ch] : 0.f;
-    const Lane<T> ldt(a.dt, a.dt_t, a.dt_b, w), lz(a.z, a.z_t, a.z_b, w), ldy(a.dy, a.dy_t, a.dy_b, w);
-    for (long long t0 = first + ((last - first - 1) / KT) * KT; t0 >= first; t0 -= KT) {
-        Rows<T, NS> rn;
-        Steps<T, J> dn, zn, gn;
-        rn.load(a, w, t0);
-        dn.load(ldt, true, t0, w.len, w.q);
-        gn.load(ldy, true, t0, w.len, w.q);
-        zn.load(lz, a.z != nullptr, t0, w.len, w.q);
-        __syncthreads();
-        rn.put(rows);
-        __syncthreads();
-        const float* lds = rows + KT * NP + w.q * NS;
+    Lane<T> ldt(a.dt, a.dt_t, a.dt_b, w, top), ldy(a.dy, a.dy_t, a.dy_b, w, top);
+    Lane<T> lz(gate ? a.z : a.dy, gate ? a.z_t : a.dy_t, gate ? a.z_b : a.dy_b, w, top);
+    Rows<T, NS> rn(a, w, top, false);
+    Steps<T, J> dn, zn, gn;
+    int rem = left_of<KT>(w.len, top);
+    auto fetch = [&]() {
+        rn.load(rem);
+        dn.load(ldt, rem, w.q);
+        gn.load(ldy, rem, w.q);
+        zn.load(lz, rem, w.q);
+    };
+    fetch();
+    rn.put(rows[0]);
+    __syncthreads();
+    int cur = 0;
+    for (long long t0 = top; t0 >= first; t0 -= KT, cur ^= 1) {
+        float e[J], g[J];
 #pragma unroll
-        for (int j = J - 1; j >= 0; --j) {
-            const float raw = to_f(dn.v[j]) + bias;
-            float e = a.softplus ? softplus_f(raw) : raw, g = to_f(gn.v[j]);
-            if (t0 + 4 * j + w.q >= w.len) e = 0.f;
-            if (a.z) {
-                const float z = to_f(zn.v[j]);
-                g *= z * sigmoid_f(z);
-            }
-            es += e;
+        for (int j = 0; j < J; ++j) {
+            const float raw = to_f(dn.v[j]) + bias, sp = softplus_f(raw), z = to_f(zn.v[j]), dy = to_f(gn.v[j]);
+            e[j] = 4 * j + w.q < rem ? (softplus ? sp : raw) : 0.f;
+            g[j] = gate ? dy * (z * sigmoid_f(z)) : dy;
+            es += e[j];
+        }
+        const bool more = t0 > first;
+        if (more) {
+            rn.move(-1);
+            ldt.move(-J);
+            ldy.move(-J);
+            lz.move(-J);
+            rem = left_of<KT>(w.len, t0 - KT);
+            fetch();
+        }
+        const float* lds = rows[cur] + KT * NP + w.q * NS;
+#pragma unroll
+        for (int j = J - 1; j >= 0; --j)
             four_back([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                const float ei = quad_bcast<i>(e), gi = quad_bcast<i>(g);
+                const float ei = quad_bcast<i>(e[j]), gi = quad_bcast<i>(g[j]);
                 const float* Ct = lds + (4 * j + i) * NP;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) q[k] = fmaf(Ct[k], gi, q[k]) * __builtin_amdgcn_exp2f(ei * A2[k]);
             });
-        }
+        if (more) rn.put(rows[cur ^ 1]);
+        __syncthreads();
     }
     es = quad_sum(es);
     if (!w.live) return;
@@ -361,9 +415,10 @@ scan_bwd_kernel(ScanArgs a) {
     __shared__ __align__(16) float rows[2 * KT * NP];
     __shared__ __align__(16) float red[WAVES][KT][2][NP];
     const Where w = where(a);
-    const bool b0 = w.q & 1, b1 = w.q & 2;
+    const bool b0 = w.q & 1, b1 = w.q & 2, softplus = a.softplus, gate = a.z != nullptr;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const long long first = (long long)blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk);
+    const long long top = last > first ? first + ((last - first - 1) / KT) * KT : first - KT;
     float A2[NS], q[NS], dA[NS], dD = 0.f, db = 0.f;
     load_A2<NS>(a, w, A2);
     load_state<NS>(a.dstate_out, a, w, q);
@@ -371,55 +426,53 @@ scan_bwd_kernel(ScanArgs a) {
 #pragma unroll
     for (int k = 0; k < NS; ++k) dA[k] = 0.f;
     const float Dv = a.D ? a.D[w.ch] : 0.f, bias = a.bias ? a.bias[w.ch] : 0.f;
-    const long long od_t = (long long)a.batch * a.d;
-    const Lane<T> lx(a.x, a.x_t, a.x_b, w), ldt(a.dt, a.dt_t, a.dt_b, w), lz(a.z, a.z_t, a.z_b, w), ldy(a.dy, a.dy_t, a.dy_b, w);
-    const Lane<T> odx(a.dx, od_t, a.d, w), oddt(a.ddt, od_t, a.d, w), odz(a.dz, od_t, a.d, w);
-    for (long long t0 = first + ((last - first - 1) / KT) * KT; t0 >= first; t0 -= KT) {
-        const bool full = t0 + KT <= w.len;
-        Rows<T, NS> rn;
+    const long long o_t = (long long)a.batch * a.d;
+    Lane<T> lx(a.x, a.x_t, a.x_b, w, top), ldt(a.dt, a.dt_t, a.dt_b, w, top), ldy(a.dy, a.dy_t, a.dy_b, w, top);
+    Lane<T> lz(gate ? a.z : a.x, gate ? a.z_t : a.x_t, gate ? a.z_b : a.x_b, w, top);
+    Lane<T> odx(a.dx, o_t, a.d, w, top), oddt(a.ddt, o_t, a.d, w, top), odz(a.dz, o_t, a.d, w, top);
+    Rows<T, NS> rn(a, w, top, true);
+    for (long long t0 = top; t0 >= first; t0 -= KT) {
+        const int rem = left_of<KT>(w.len, t0), there = left_of<KT>(a.steps, t0);
         Steps<T, J> xn, dn, zn, gn;
-        rn.load(a, w, t0);
+        rn.load(rem);
         const Part<NS> h0 = *part_at<NS>(a.ckpt, a, w, t0 / KT);
-        xn.load(lx, true, t0, w.len, w.q);
-        dn.load(ldt, true, t0, w.len, w.q);
-        gn.load(ldy, true, t0, w.len, w.q);
-        zn.load(lz, a.z != nullptr, t0, w.len, w.q);
+        xn.load(lx, rem, w.q);
+        dn.load(ldt, rem, w.q);
+        gn.load(ldy, rem, w.q);
+        zn.load(lz, rem, w.q);
         float x[J], e[J], raw[J], g[J], hs[KT][NS], as[KT][NS];
         rn.put(rows);
         __syncthreads();
         const float* lds = rows + w.q * NS;
         // the tile's states once more, and the output in front of the gate
+        float dz[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             x[j] = w.live ? to_f(xn.v[j]) : 0.f;
             raw[j] = to_f(dn.v[j]) + bias;
-            e[j] = a.softplus ? softplus_f(raw[j]) : raw[j];
-            if (!full && t0 + 4 * j + w.q >= w.len) e[j] = 0.f;
+            const float sp = softplus_f(raw[j]);
+            e[j] = 4 * j + w.q < rem ? (softplus ? sp : raw[j]) : 0.f;
             const float dy = w.live ? to_f(gn.v[j]) : 0.f, u = e[j] * x[j];
             float p[4];
             four([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                const int s = 4 * j + i;
+                const int t = 4 * j + i;
                 const float ei = quad_bcast<i>(e[j]), ui = quad_bcast<i>(u);
-                const float *Bt = lds + s * NP, *Ct = Bt + KT * NP;
+                const float *Bt = lds + t * NP, *Ct = Bt + KT * NP;
                 p[i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
-                    as[s][k] = __builtin_amdgcn_exp2f(ei * A2[k]);
-                    hs[s][k] = fmaf(as[s][k], s > 0 ? hs[s > 0 ? s - 1 : 0][k] : h0.v[k], ui * Bt[k]);
-                    p[i] = fmaf(Ct[k], hs[s][k], p[i]);
+                    as[t][k] = __builtin_amdgcn_exp2f(ei * A2[k]);
+                    hs[t][k] = fmaf(as[t][k], t > 0 ? hs[t > 0 ? t - 1 : 0][k] : h0.v[k], ui * Bt[k]);
+                    p[i] = fmaf(Ct[k], hs[t][k], p[i]);
                 }
             });
-            const float pre = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
-            g[j] = dy;
-            if (a.z) {
-                const float z = to_f(zn.v[j]), sg = sigmoid_f(z);
-                g[j] = dy * z * sg;
-                const long long t = t0 + 4 * j + w.q;
-                if (w.live && (full || t < a.steps)) odz.store(t0 + 4 * j, full || t < w.len ? dy * pre * sg * (1.f + z * (1.f - sg)) : 0.f);
-            }
+            const float pre = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1)), z = to_f(zn.v[j]), sg = sigmoid_f(z);
+            g[j] = gate ? dy * (z * sg) : dy;
+            dz[j] = dy * pre * (sg * (1.f + z * (1.f - sg)));
             dD = fmaf(g[j], x[j], dD);
         }
+        if (gate && w.live) odz.template store_tile<J>(dz, rem, there, w.q);
         float dAt[NS];
 #pragma unroll
         for (int k = 0; k < NS; ++k) dAt[k] = 0.f;
@@ -429,18 +482,18 @@ scan_bwd_kernel(ScanArgs a) {
             const float u = e[j] * x[j];
             four_back([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                const int s = 4 * j + i;
+                const int t = 4 * j + i;
                 const float gi = quad_bcast<i>(g[j]), ui = quad_bcast<i>(u), ei = quad_bcast<i>(e[j]);
-                const float *Bt = lds + s * NP, *Ct = Bt + KT * NP;
+                const float *Bt = lds + t * NP, *Ct = Bt + KT * NP;
                 pb[i] = pf[i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
                     q[k] = fmaf(Ct[k], gi, q[k]);
                     pb[i] = fmaf(q[k], Bt[k], pb[i]);
                     v[i * NS + k] = q[k] * ui;
-                    v[(4 + i) * NS + k] = gi * hs[s][k];
-                    q[k] *= as[s][k];
-                    const float f = q[k] * (s > 0 ? hs[s > 0 ? s - 1 : 0][k] : h0.v[k]);
+                    v[(4 + i) * NS + k] = gi * hs[t][k];
+                    q[k] *= as[t][k];
+                    const float f = q[k] * (t > 0 ? hs[t > 0 ? t - 1 : 0][k] : h0.v[k]);
                     dAt[k] = fmaf(f, ei, dAt[k]);
                     pf[i] = fmaf(f, A2[k], pf[i]);
                 }
@@ -452,15 +505,14 @@ scan_bwd_kernel(ScanArgs a) {
                 for (int k = 0; k < HALF; ++k) to[k] = v[k];       // (NS = 1: both lanes write the same sum)
             }
             const float qb = quad_scatter_sum(pb, b0, b1), fa = quad_scatter_sum(pf, b0, b1) * LN2_F;
-            const long long t = t0 + 4 * j + w.q;
-            float de = fmaf(qb, x[j], fa);
-            if (a.softplus) de *= sigmoid_f(raw[j]);
-            if (!full && t >= w.len) de = 0.f;
-            db += de;
-            if (w.live && (full || t < a.steps)) {
-                odx.store(t0 + 4 * j, full || t < w.len ? fmaf(g[j], Dv, qb * e[j]) : 0.f);
-                oddt.store(t0 + 4 * j, de);
-            }
+            const float de = fmaf(qb, x[j], fa), sl = sigmoid_f(raw[j]);
+            raw[j] = 4 * j + w.q < rem ? (softplus ? de * sl : de) : 0.f;              // now the gradient of dt
+            db += raw[j];
+            x[j] = fmaf(g[j], Dv, qb * e[j]);                                          // now the gradient of x
+        }
+        if (w.live) {
+            odx.template store_tile<J>(x, rem, there, w.q);
+            oddt.template store_tile<J>(raw, rem, there, w.q);
         }
 #pragma unroll
         for (int k = 0; k < NS; ++k) dA[k] += dAt[k];
@@ -470,9 +522,17 @@ scan_bwd_kernel(ScanArgs a) {
             float s = 0.f;
 #pragma unroll
             for (int v = 0; v < WAVES; ++v) s += (&red[v][0][0][0])[i];
-            if (t0 + t < a.steps)
+            if (t < there)
                 a.part_bc[((((long long)w.tile * a.steps + t0 + t) * a.batch + w.b) * a.groups + w.g) * 2 * NP + i % (2 * NP)] = s;
         }
+        rn.move(-1);
+        lx.move(-J);
+        ldt.move(-J);
+        ldy.move(-J);
+        lz.move(-J);
+        odx.move(-J);
+        oddt.move(-J);
+        odz.move(-J);
     }
     if (blockIdx.z == 0) store_state<NS>(a.dstate0, a, w, q);
     dD = quad_sum(dD);
