@@ -88,12 +88,6 @@ __device__ __forceinline__ unsigned block_prefix(unsigned v, unsigned* wsum) {
     return before + s - v;
 }
 
-// LDS accesses of a wave's lanes on either side stay on theirs (the hardware keeps a wave's LDS operations in order)
-__device__ __forceinline__ void wave_order() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 // Ranks one round of items: every wave owns consecutive ones; equal digits of 64 items find each other by one ballot per digit
 // bit, so an item's rank is (earlier ones of its wave) + (peers in lower lanes), without atomics.  Leaves each wave's counts.
 __device__ __forceinline__ void rank_round(const SortArgs& a, long long r0, long long hi, unsigned (*wcnt)[RADIX], uint2* item, unsigned* rank) {

@@ -15,8 +15,11 @@
 namespace {
 
 constexpr int WAVES = 4, CH = 16 * WAVES;              // channels of a workgroup
-constexpr int MAX_CHUNKS = 64, FWD_TARGET = 1024, BWD_TARGET = 512;
-template <int NS> struct Tile { static constexpr int KT = NS <= 4 ? 16 : 8; };      // steps between saved states
+constexpr int MAX_CHUNKS = 64, FWD_TARGET = 2048, BWD_TARGET = 768;
+// Steps of a tile: the forward passes take 16 (loads, address arithmetic and the barrier are shared by more steps), the backward pass
+// 8, whose states fit the registers of three waves a SIMD; states are saved every 8 steps.  (16 and two waves: 565 against
+// 450 us on 2048 x 8 x 2048; 32 states need twice the registers a step, so 8 in all passes.)
+template <int NS> struct Tile { static constexpr int KT = NS <= 4 ? 16 : 8, BACK = 8; };
 
 struct ScanArgs {
     const void *x, *dt, *B, *C, *z, *dy;
@@ -28,7 +31,7 @@ struct ScanArgs {
     float *part_bc, *part_a, *part_d;                  // partial sums of dB | dC, dA, dD | dbias
     const int* lengths;
     long long x_t, x_b, dt_t, dt_b, z_t, z_b, B_t, B_b, B_g, C_t, C_b, C_g, dy_t, dy_b;
-    long long steps, chunk;                            // steps of a chunk (blockIdx.z), a multiple of KT
+    int steps, chunk;                                  // steps of a chunk (blockIdx.z), a multiple of KT
     int batch, d, groups, n, softplus;
 };
 
@@ -52,7 +55,7 @@ __device__ __forceinline__ float quad_scatter_sum(const float* p, bool b0, bool 
 struct Where {
     int b, g, ch, q, tile;                             // channel (global), lane of the quad, channel tile of the group
     bool live;                                         // the channel exists
-    long long len;
+    int len;
 };
 __device__ __forceinline__ Where where(const ScanArgs& a) {
     Where w;
@@ -64,8 +67,7 @@ __device__ __forceinline__ Where where(const ScanArgs& a) {
     const int c = w.tile * CH + (threadIdx.x >> 2);
     w.live = c < dg;
     w.ch = w.g * dg + (w.live ? c : 0);
-    long long n = a.lengths ? a.lengths[w.b] : a.steps;
-    w.len = n < 0 ? 0 : n > a.steps ? a.steps : n;
+    w.len = a.lengths ? min(max(a.lengths[w.b], 0), a.steps) : a.steps;
     return w;
 }
 
@@ -74,14 +76,14 @@ __device__ __forceinline__ Where where(const ScanArgs& a) {
 // are checked on the host: lane_ok).
 template <typename T> struct Lane {
     const char* at;                                    // of the tile, batch element b
-    long long step4;                                   // bytes of four steps
+    unsigned step4;                                    // bytes of four steps
     unsigned off;                                      // (q * step + channel), bytes
-    __device__ __forceinline__ Lane(const void* p, long long s_t, long long s_b, const Where& w, long long t0)
-        : at((const char*)p + (t0 * s_t + w.b * s_b) * (long long)sizeof(T)), step4(4 * s_t * (long long)sizeof(T)),
+    __device__ __forceinline__ Lane(const void* p, long long s_t, long long s_b, const Where& w, int t0)
+        : at((const char*)p + (t0 * s_t + w.b * s_b) * (long long)sizeof(T)), step4(4u * (unsigned)s_t * (unsigned)sizeof(T)),
           off((unsigned)(w.q * s_t + w.ch) * (unsigned)sizeof(T)) {}
     __device__ __forceinline__ T load(int j) const { return *(const T*)(at + j * step4 + off); }
     __device__ __forceinline__ void store(int j, float v) const { *(T*)(const_cast<char*>(at) + j * step4 + off) = from_f<T>(v); }
-    __device__ __forceinline__ void move(int tiles_j) { at += tiles_j * step4; }
+    __device__ __forceinline__ void move(int j) { at += (long long)step4 * j; }
     // values of a tile's steps, those before `rem` (of the sequence) as computed, the others (of the tensor) as zeros
     template <int J> __device__ __forceinline__ void store_tile(const float* v, int rem, int there, int q) const {
         if (rem >= 4 * J) {
@@ -95,9 +97,11 @@ template <typename T> struct Lane {
     }
 };
 // steps of a tile that are left of `len`
-template <int KT> __device__ __forceinline__ int left_of(long long len, long long t0) {
-    const long long r = len - t0;
-    return r >= KT ? KT : r < 0 ? 0 : (int)r;
+template <int KT> __device__ __forceinline__ int left_of(int len, int t0) { return min(max(len - t0, 0), KT); }
+// values of steps behind the sequence's end -> 0
+template <int J> __device__ __forceinline__ void cut_steps(float* v, int rem, int q) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) v[j] = 4 * j + q < rem ? v[j] : 0.f;
 }
 // a tile's values as stored; steps behind the end are not touched
 template <typename T, int J> struct Steps {
@@ -114,14 +118,14 @@ template <typename T, int J> struct Steps {
 };
 
 // a tile's rows of B and C -> LDS, fp32, zero behind the sequence and in the padded states
-template <typename T, int NS>
+template <typename T, int NS, int KT>
 struct Rows {
-    static constexpr int KT = Tile<NS>::KT, NP = 4 * NS, PER = (2 * KT * NP + 255) / 256;
+    static constexpr int NP = 4 * NS, PER = (2 * KT * NP + 255) / 256;
     T v[PER];
     const char* at[PER];
     long long tile[PER];                               // bytes of a tile
     int t[PER];                                        // step within the tile; KT: nothing to load
-    __device__ __forceinline__ Rows(const ScanArgs& a, const Where& w, long long t0, bool with_B) {
+    __device__ __forceinline__ Rows(const ScanArgs& a, const Where& w, int t0, bool with_B) {
 #pragma unroll
         for (int r = 0; r < PER; ++r) {
             const int i = threadIdx.x + 256 * r, n = i % NP;
@@ -198,8 +202,9 @@ template <typename F> __device__ __forceinline__ void four_back(F f) {
     f(std::integral_constant<int, 0>());
 }
 
-// The loops below have no branch between a tile's loads and its stores: options (softplus, the gate) are selects, without z its
-// loads read x.
+// The loops below have no branch between a tile's loads and its stores: options (softplus, the gate) are selects (pick keeps the
+// compiler from making branches of them), without z its loads read x.
+#define pick(c) __builtin_unpredictable(c)
 
 // LOCAL: the chunk's own contribution to the state (from zero) and its sum of e, for carry_in
 template <typename T, int NS, bool LOCAL>
@@ -209,7 +214,7 @@ scan_fwd_kernel(ScanArgs a) {
     __shared__ __align__(16) float rows[2][2 * KT * NP];
     const Where w = where(a);
     const bool b0 = w.q & 1, b1 = w.q & 2, softplus = a.softplus, gate = a.z != nullptr;
-    const long long first = (long long)blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk);
+    const int first = blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk), end = min(last, max(first, w.len));
     float A2[NS], h[NS], es = 0.f;
     load_A2<NS>(a, w, A2);
     if (LOCAL) {
@@ -222,7 +227,7 @@ scan_fwd_kernel(ScanArgs a) {
     const float Dv = a.D ? a.D[w.ch] : 0.f, bias = a.bias ? a.bias[w.ch] : 0.f;
     Lane<T> lx(a.x, a.x_t, a.x_b, w, first), ldt(a.dt, a.dt_t, a.dt_b, w, first);
     Lane<T> lz(gate ? a.z : a.x, gate ? a.z_t : a.x_t, gate ? a.z_b : a.x_b, w, first), ly(a.y, (long long)a.batch * a.d, a.d, w, first);
-    Rows<T, NS> rn(a, w, first, true);
+    Rows<T, NS, KT> rn(a, w, first, true);
     Steps<T, J> xn, dn, zn;
     int rem = left_of<KT>(w.len, first);
     auto fetch = [&]() {
@@ -234,18 +239,25 @@ scan_fwd_kernel(ScanArgs a) {
     fetch();
     rn.put(rows[0]);
     __syncthreads();
+    Part<NS>* ck = (!LOCAL && a.ckpt && w.live) ? part_at<NS>(a.ckpt, a, w, first / Tile<NS>::BACK) : nullptr;
+    const long long ck_tile = (long long)a.batch * a.d * 4;
     int cur = 0;
-    for (long long t0 = first; t0 < last; t0 += KT, cur ^= 1) {
-        float x[J], e[J], z[J], y[J];
+    int t0 = first;
+    for (; t0 < end; t0 += KT, cur ^= 1) {
+        float x[J], e[J], gz[J], y[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             x[j] = to_f(xn.v[j]);
             const float raw = to_f(dn.v[j]) + bias, sp = softplus_f(raw);
-            e[j] = 4 * j + w.q < rem ? (softplus ? sp : raw) : 0.f;
-            if (!LOCAL) z[j] = to_f(zn.v[j]);
+            e[j] = pick(softplus) ? sp : raw;
+            if (!LOCAL) {
+                const float z = to_f(zn.v[j]), zs = z * sigmoid_f(z);
+                gz[j] = pick(gate) ? zs : 1.f;
+            }
         }
+        if (rem < KT) cut_steps<J>(e, rem, w.q);
         const int now = rem;
-        const bool more = t0 + KT < last;
+        const bool more = t0 + KT < end;
         if (more) {
             rn.move(1);
             lx.move(J);
@@ -254,18 +266,19 @@ scan_fwd_kernel(ScanArgs a) {
             rem = left_of<KT>(w.len, t0 + KT);
             fetch();
         }
-        if (!LOCAL && a.ckpt && w.live) {
-            Part<NS> p;
-#pragma unroll
-            for (int k = 0; k < NS; ++k) p.v[k] = h[k];
-            *part_at<NS>(a.ckpt, a, w, t0 / KT) = p;
-        }
         const float* lds = rows[cur] + w.q * NS;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             float p[4];
             const float u = e[j] * x[j];
             if (LOCAL) es += e[j];
+            if (!LOCAL && ck && (4 * j) % Tile<NS>::BACK == 0 && t0 + 4 * j < a.steps) {
+                Part<NS> c;
+#pragma unroll
+                for (int k = 0; k < NS; ++k) c.v[k] = h[k];
+                *ck = c;
+                ck += ck_tile;
+            }
             four([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const float ei = quad_bcast<i>(e[j]), ui = quad_bcast<i>(u);
@@ -277,10 +290,7 @@ scan_fwd_kernel(ScanArgs a) {
                     if (!LOCAL) p[i] = fmaf(Ct[k], h[k], p[i]);
                 }
             });
-            if (!LOCAL) {
-                const float v = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
-                y[j] = gate ? v * (z[j] * sigmoid_f(z[j])) : v;
-            }
+            if (!LOCAL) y[j] = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1)) * gz[j];
         }
         if (!LOCAL) {
             if (w.live) ly.template store_tile<J>(y, now, left_of<KT>(a.steps, t0), w.q);
@@ -288,6 +298,10 @@ scan_fwd_kernel(ScanArgs a) {
         }
         if (more) rn.put(rows[cur ^ 1]);
         __syncthreads();
+    }
+    if (!LOCAL && w.live) {                            // tiles behind the sequence's end
+        const float none[J] = {};
+        for (; t0 < last; t0 += KT, ly.move(J)) ly.template store_tile<J>(none, 0, left_of<KT>(a.steps, t0), w.q);
     }
     if (LOCAL) {
         es = quad_sum(es);
@@ -311,7 +325,8 @@ scan_adjoint_kernel(ScanArgs a) {
     const Where w = where(a);
     const bool softplus = a.softplus, gate = a.z != nullptr;
     const int chunk = blockIdx.z + 1;                  // nothing is in front of chunk 0
-    const long long first = (long long)chunk * a.chunk, last = min(a.steps, first + a.chunk), top = first + ((last - first - 1) / KT) * KT;
+    const int first = chunk * a.chunk, end = min(min(a.steps, first + a.chunk), max(first, w.len));
+    const int top = end > first ? first + ((end - first - 1) / KT) * KT : first - KT;
     float A2[NS], q[NS], es = 0.f;
     load_A2<NS>(a, w, A2);
 #pragma unroll
@@ -319,7 +334,7 @@ scan_adjoint_kernel(ScanArgs a) {
     const float bias = a.bias ? a.bias[w.ch] : 0.f;
     Lane<T> ldt(a.dt, a.dt_t, a.dt_b, w, top), ldy(a.dy, a.dy_t, a.dy_b, w, top);
     Lane<T> lz(gate ? a.z : a.dy, gate ? a.z_t : a.dy_t, gate ? a.z_b : a.dy_b, w, top);
-    Rows<T, NS> rn(a, w, top, false);
+    Rows<T, NS, KT> rn(a, w, top, false);
     Steps<T, J> dn, zn, gn;
     int rem = left_of<KT>(w.len, top);
     auto fetch = [&]() {
@@ -328,19 +343,22 @@ scan_adjoint_kernel(ScanArgs a) {
         gn.load(ldy, rem, w.q);
         zn.load(lz, rem, w.q);
     };
-    fetch();
-    rn.put(rows[0]);
+    if (top >= first) {
+        fetch();
+        rn.put(rows[0]);
+    }
     __syncthreads();
     int cur = 0;
-    for (long long t0 = top; t0 >= first; t0 -= KT, cur ^= 1) {
+    for (int t0 = top; t0 >= first; t0 -= KT, cur ^= 1) {
         float e[J], g[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             const float raw = to_f(dn.v[j]) + bias, sp = softplus_f(raw), z = to_f(zn.v[j]), dy = to_f(gn.v[j]);
-            e[j] = 4 * j + w.q < rem ? (softplus ? sp : raw) : 0.f;
-            g[j] = gate ? dy * (z * sigmoid_f(z)) : dy;
-            es += e[j];
+            const float zs = z * sigmoid_f(z);
+            e[j] = pick(softplus) ? sp : raw;
+            g[j] = dy * (pick(gate) ? zs : 1.f);
         }
+        if (rem < KT) cut_steps<J>(e, rem, w.q);
         const bool more = t0 > first;
         if (more) {
             rn.move(-1);
@@ -352,7 +370,8 @@ scan_adjoint_kernel(ScanArgs a) {
         }
         const float* lds = rows[cur] + KT * NP + w.q * NS;
 #pragma unroll
-        for (int j = J - 1; j >= 0; --j)
+        for (int j = J - 1; j >= 0; --j) {
+            es += e[j];
             four_back([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const float ei = quad_bcast<i>(e[j]), gi = quad_bcast<i>(g[j]);
@@ -360,6 +379,7 @@ scan_adjoint_kernel(ScanArgs a) {
 #pragma unroll
                 for (int k = 0; k < NS; ++k) q[k] = fmaf(Ct[k], gi, q[k]) * __builtin_amdgcn_exp2f(ei * A2[k]);
             });
+        }
         if (more) rn.put(rows[cur ^ 1]);
         __syncthreads();
     }
@@ -372,53 +392,54 @@ scan_adjoint_kernel(ScanArgs a) {
     if (w.q == 0) a.esum[((long long)chunk * a.batch + w.b) * a.d + w.ch] = es;
 }
 
-__device__ __forceinline__ unsigned bits(float v) { return __builtin_bit_cast(unsigned, v); }
-__device__ __forceinline__ float swap32_sum(float a, float b) {        // lanes 0-31: a over both halves, lanes 32-63: b
-    const auto r = __builtin_amdgcn_permlane32_swap(bits(a), bits(b), false, false);
-    const unsigned lo = r[0], hi = r[1];               // (bit_cast of a vector's element reads element 0)
-    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-}
-__device__ __forceinline__ float swap16_sum(float a, float b) {        // even rows of 16 lanes: a over a pair of rows, odd rows: b
-    const auto r = __builtin_amdgcn_permlane16_swap(bits(a), bits(b), false, false);
-    const unsigned lo = r[0], hi = r[1];
-    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
-}
-// Sums over the wave's 16 channels of v[2][4][NS] (dB | dC, step, state): halved four times, every halving one exchange of
-// lanes and one addition a pair.  Lane l is left with kind l5, step (l4, l3) and the max(NS / 2, 1) states from l2 NS / 2.
-template <int NS> __device__ __forceinline__ void channel_sums(float* v, int lane) {
+// Sums over the wave's 16 channels of v[2][4][NS] (dB | dC, step, state), through the wave's own piece of LDS: written as
+// [kind, step][channel][4 NS states], read back across the channels.  Lane l adds for (kind, step) = l >> 3 the four states from
+// 4 (l & 7) / SPLIT over a SPLIT-th of the channels, then SPLIT neighbouring lanes add up.  (Halving the values by lane exchanges
+// instead, 24 permlane swaps and their additions for 4 steps, took 90 issue slots against 32: the vector ALUs bound this kernel.)
+template <int NS> struct Sums {
+    static constexpr int NP = 4 * NS, SPLIT = 8 / NS, EACH = 16 / SPLIT;
+    // (16 floats more behind every EACH channels: the SPLIT lanes that read next to each other meet different banks)
+    static constexpr int PART = EACH * NP + 16, PITCH = SPLIT * PART;
+    float lds[8 * PITCH];
+    __device__ __forceinline__ void put(int block, int lane, const float* v) {
+        Part<NS> p;
 #pragma unroll
-    for (int i = 0; i < 4 * NS; ++i) v[i] = swap32_sum(v[i], v[i + 4 * NS]);
-#pragma unroll
-    for (int i = 0; i < 2 * NS; ++i) v[i] = swap16_sum(v[i], v[i + 2 * NS]);
-    const bool l3 = lane & 8, l2 = lane & 4;
-#pragma unroll
-    for (int i = 0; i < NS; ++i) {
-        const float lo = v[i] + dpp<0x128>(v[i]), hi = v[i + NS] + dpp<0x128>(v[i + NS]);        // row_ror:8 = the lane with bit 3 flipped
-        v[i] = l3 ? hi : lo;
+        for (int k = 0; k < NS; ++k) p.v[k] = v[k];
+        *reinterpret_cast<Part<NS>*>(&lds[block * PITCH + (lane / (4 * EACH)) * PART + (lane % (4 * EACH)) * NS]) = p;
     }
-    if (NS == 1) {
-        const float lo = v[0] + dpp<0x104>(v[0]), hi = v[0] + dpp<0x114>(v[0]);                  // row_shl:4, row_shr:4
-        v[0] = l2 ? hi : lo;
-    } else {
+    // -> this lane's four states' sums; block l >> 3, states from 4 * ((l & 7) / SPLIT)
+    __device__ __forceinline__ f32x4 take(int lane) const {
+        const float* at = &lds[(lane >> 3) * PITCH + (lane & (SPLIT - 1)) * PART + 4 * ((lane & 7) / SPLIT)];
+        f32x4 s = *reinterpret_cast<const f32x4*>(at);
 #pragma unroll
-        for (int i = 0; i < NS / 2; ++i) {
-            const float lo = v[i] + dpp<0x104>(v[i]), hi = v[i + NS / 2] + dpp<0x114>(v[i + NS / 2]);
-            v[i] = l2 ? hi : lo;
+        for (int c = 1; c < EACH; ++c) s += *reinterpret_cast<const f32x4*>(at + c * NP);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float v = s[i];
+            if (SPLIT >= 2) v += quad_xor1(v);
+            if (SPLIT >= 4) v += quad_xor2(v);
+            if (SPLIT >= 8) {
+                const float lo = dpp<0x104>(v), hi = dpp<0x114>(v);      // row_shl:4, row_shr:4: the lane with bit 2 flipped
+                v += (lane & 4) ? hi : lo;
+            }
+            s[i] = v;
         }
+        return s;
     }
-}
+};
 
 template <typename T, int NS>
-__global__ void __launch_bounds__(256, 2)
+__global__ void __launch_bounds__(256, NS == 8 ? 1 : 3)
 scan_bwd_kernel(ScanArgs a) {
-    constexpr int KT = Tile<NS>::KT, NP = 4 * NS, J = KT / 4, HALF = NS > 1 ? NS / 2 : 1;
-    __shared__ __align__(16) float rows[2 * KT * NP];
-    __shared__ __align__(16) float red[WAVES][KT][2][NP];
+    constexpr int KT = Tile<NS>::BACK, NP = 4 * NS, J = KT / 4;
+    __shared__ __align__(16) float rows[2][2 * KT * NP];
+    __shared__ __align__(16) float red[2][WAVES][2][KT][NP];
+    __shared__ __align__(16) Sums<NS> sums[WAVES];
     const Where w = where(a);
     const bool b0 = w.q & 1, b1 = w.q & 2, softplus = a.softplus, gate = a.z != nullptr;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const long long first = (long long)blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk);
-    const long long top = last > first ? first + ((last - first - 1) / KT) * KT : first - KT;
+    const int first = blockIdx.z * a.chunk, last = min(a.steps, first + a.chunk), end = min(last, max(first, w.len));
+    const int top = end > first ? first + ((end - first - 1) / KT) * KT : first - KT;
     float A2[NS], q[NS], dA[NS], dD = 0.f, db = 0.f;
     load_A2<NS>(a, w, A2);
     load_state<NS>(a.dstate_out, a, w, q);
@@ -430,29 +451,73 @@ scan_bwd_kernel(ScanArgs a) {
     Lane<T> lx(a.x, a.x_t, a.x_b, w, top), ldt(a.dt, a.dt_t, a.dt_b, w, top), ldy(a.dy, a.dy_t, a.dy_b, w, top);
     Lane<T> lz(gate ? a.z : a.x, gate ? a.z_t : a.x_t, gate ? a.z_b : a.x_b, w, top);
     Lane<T> odx(a.dx, o_t, a.d, w, top), oddt(a.ddt, o_t, a.d, w, top), odz(a.dz, o_t, a.d, w, top);
-    Rows<T, NS> rn(a, w, top, true);
-    for (long long t0 = top; t0 >= first; t0 -= KT) {
-        const int rem = left_of<KT>(w.len, t0), there = left_of<KT>(a.steps, t0);
-        Steps<T, J> xn, dn, zn, gn;
+    Rows<T, NS, KT> rn(a, w, top, true);
+    const Part<NS>* ck = part_at<NS>(a.ckpt, a, w, top / KT);
+    const long long ck_tile = (long long)a.batch * a.d * 4, bc_tile = (long long)KT * a.batch * a.groups * 2 * NP;
+    constexpr int PER = (2 * KT * NP + 255) / 256;
+    float* bc[PER];                                    // where this thread's sums of the tile go
+    int bc_t[PER];
+#pragma unroll
+    for (int r = 0; r < PER; ++r) {
+        const int i = threadIdx.x + 256 * r;
+        bc_t[r] = i < 2 * KT * NP ? (i / NP) % KT : KT;
+        bc[r] = a.part_bc + ((((long long)w.tile * a.steps + top + (i / NP) % KT) * a.batch + w.b) * a.groups + w.g) * 2 * NP + i / (KT * NP) * NP + i % NP;
+    }
+    {                                                  // tiles behind the sequence's end: no gradient
+        const float none[J] = {};
+        Lane<T> zx = odx, zdt = oddt, zz = odz;
+        for (int t0 = top + KT, k = 1; t0 < last; t0 += KT, ++k) {
+            const int there = left_of<KT>(a.steps, t0);
+            zx.move(J);
+            zdt.move(J);
+            zz.move(J);
+            if (w.live) {
+                zx.template store_tile<J>(none, 0, there, w.q);
+                zdt.template store_tile<J>(none, 0, there, w.q);
+                if (gate) zz.template store_tile<J>(none, 0, there, w.q);
+            }
+#pragma unroll
+            for (int r = 0; r < PER; ++r)
+                if (bc_t[r] < there) bc[r][k * bc_tile] = 0.f;
+        }
+    }
+    Steps<T, J> xn, dn, zn, gn;
+    Part<NS> h0n;
+    int rem = left_of<KT>(w.len, top);
+    auto fetch = [&]() {
         rn.load(rem);
-        const Part<NS> h0 = *part_at<NS>(a.ckpt, a, w, t0 / KT);
+        h0n = *ck;
         xn.load(lx, rem, w.q);
         dn.load(ldt, rem, w.q);
         gn.load(ldy, rem, w.q);
         zn.load(lz, rem, w.q);
-        float x[J], e[J], raw[J], g[J], hs[KT][NS], as[KT][NS];
-        rn.put(rows);
-        __syncthreads();
-        const float* lds = rows + w.q * NS;
-        // the tile's states once more, and the output in front of the gate
-        float dz[J];
+    };
+    if (top >= first) {
+        fetch();
+        rn.put(rows[0]);
+    }
+    __syncthreads();
+    int cur = 0;
+    for (int t0 = top; t0 >= first; t0 -= KT, cur ^= 1) {
+        const int now = rem, there = left_of<KT>(a.steps, t0);
+        const bool more = t0 > first;
+        float x[J], e[J], raw[J], g[J], dz[J], hs[KT][NS], as[KT][NS];
+        const Part<NS> h0 = h0n;
+        const float* lds = rows[cur] + w.q * NS;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
             x[j] = w.live ? to_f(xn.v[j]) : 0.f;
             raw[j] = to_f(dn.v[j]) + bias;
-            const float sp = softplus_f(raw[j]);
-            e[j] = 4 * j + w.q < rem ? (softplus ? sp : raw[j]) : 0.f;
-            const float dy = w.live ? to_f(gn.v[j]) : 0.f, u = e[j] * x[j];
+            const float sp = softplus_f(raw[j]), dy = w.live ? to_f(gn.v[j]) : 0.f, z = to_f(zn.v[j]), sg = sigmoid_f(z), zs = z * sg;
+            e[j] = pick(softplus) ? sp : raw[j];
+            g[j] = dy * (pick(gate) ? zs : 1.f);
+            dz[j] = dy * (sg * (1.f + z * (1.f - sg)));
+        }
+        if (now < KT) cut_steps<J>(e, now, w.q);
+        // the tile's states once more, and the output in front of the gate
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+            const float u = e[j] * x[j];
             float p[4];
             four([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
@@ -467,69 +532,80 @@ scan_bwd_kernel(ScanArgs a) {
                     p[i] = fmaf(Ct[k], hs[t][k], p[i]);
                 }
             });
-            const float pre = fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1)), z = to_f(zn.v[j]), sg = sigmoid_f(z);
-            g[j] = gate ? dy * (z * sg) : dy;
-            dz[j] = dy * pre * (sg * (1.f + z * (1.f - sg)));
+            dz[j] *= fmaf(Dv, x[j], quad_scatter_sum(p, b0, b1));
             dD = fmaf(g[j], x[j], dD);
         }
-        if (gate && w.live) odz.template store_tile<J>(dz, rem, there, w.q);
+        if (gate && w.live) odz.template store_tile<J>(dz, now, there, w.q);
         float dAt[NS];
 #pragma unroll
         for (int k = 0; k < NS; ++k) dAt[k] = 0.f;
 #pragma unroll
         for (int j = J - 1; j >= 0; --j) {
-            float pb[4], pf[4], v[8 * NS];
+            float pb[4], pf[4];
             const float u = e[j] * x[j];
             four_back([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
                 const int t = 4 * j + i;
                 const float gi = quad_bcast<i>(g[j]), ui = quad_bcast<i>(u), ei = quad_bcast<i>(e[j]);
                 const float *Bt = lds + t * NP, *Ct = Bt + KT * NP;
+                float vb[NS], vc[NS];
                 pb[i] = pf[i] = 0.f;
 #pragma unroll
                 for (int k = 0; k < NS; ++k) {
                     q[k] = fmaf(Ct[k], gi, q[k]);
                     pb[i] = fmaf(q[k], Bt[k], pb[i]);
-                    v[i * NS + k] = q[k] * ui;
-                    v[(4 + i) * NS + k] = gi * hs[t][k];
+                    vb[k] = q[k] * ui;
+                    vc[k] = gi * hs[t][k];
                     q[k] *= as[t][k];
                     const float f = q[k] * (t > 0 ? hs[t > 0 ? t - 1 : 0][k] : h0.v[k]);
                     dAt[k] = fmaf(f, ei, dAt[k]);
                     pf[i] = fmaf(f, A2[k], pf[i]);
                 }
+                sums[wave].put(i, lane, vb);
+                sums[wave].put(4 + i, lane, vc);
             });
-            channel_sums<NS>(v, lane);
-            {
-                float* to = &red[wave][4 * j + ((lane >> 3) & 3)][lane >> 5][w.q * NS + (NS > 1 && (lane & 4) ? NS / 2 : 0)];
-#pragma unroll
-                for (int k = 0; k < HALF; ++k) to[k] = v[k];       // (NS = 1: both lanes write the same sum)
-            }
+            wave_fence();
+            const f32x4 bc_sum = sums[wave].take(lane);
             const float qb = quad_scatter_sum(pb, b0, b1), fa = quad_scatter_sum(pf, b0, b1) * LN2_F;
             const float de = fmaf(qb, x[j], fa), sl = sigmoid_f(raw[j]);
-            raw[j] = 4 * j + w.q < rem ? (softplus ? de * sl : de) : 0.f;              // now the gradient of dt
-            db += raw[j];
+            raw[j] = de * (pick(softplus) ? sl : 1.f);                                 // now the gradient of dt
             x[j] = fmaf(g[j], Dv, qb * e[j]);                                          // now the gradient of x
+            // (SPLIT lanes hold and write the same sums)
+            *reinterpret_cast<f32x4*>(&red[cur][wave][lane >> 5][4 * j + ((lane >> 3) & 3)][4 * ((lane & 7) / Sums<NS>::SPLIT)]) = bc_sum;
+            wave_fence();
+            if (j == J / 2 && more) {                  // half of the tile's registers are free: the next one's loads
+                rn.move(-1);
+                ck -= ck_tile;
+                lx.move(-J);
+                ldt.move(-J);
+                ldy.move(-J);
+                lz.move(-J);
+                rem = left_of<KT>(w.len, t0 - KT);
+                fetch();
+            }
         }
+        if (now < KT) cut_steps<J>(raw, now, w.q);
+#pragma unroll
+        for (int j = 0; j < J; ++j) db += raw[j];
         if (w.live) {
-            odx.template store_tile<J>(x, rem, there, w.q);
-            oddt.template store_tile<J>(raw, rem, there, w.q);
+            odx.template store_tile<J>(x, now, there, w.q);
+            oddt.template store_tile<J>(raw, now, there, w.q);
         }
 #pragma unroll
         for (int k = 0; k < NS; ++k) dA[k] += dAt[k];
-        __syncthreads();
-        for (int i = threadIdx.x; i < KT * 2 * NP; i += 256) {
-            const int t = i / (2 * NP);
-            float s = 0.f;
+        if (more) rn.put(rows[cur ^ 1]);
+        __syncthreads();                               // (red and rows have two sides: one barrier a tile)
 #pragma unroll
-            for (int v = 0; v < WAVES; ++v) s += (&red[v][0][0][0])[i];
-            if (t < there)
-                a.part_bc[((((long long)w.tile * a.steps + t0 + t) * a.batch + w.b) * a.groups + w.g) * 2 * NP + i % (2 * NP)] = s;
+        for (int r = 0; r < PER; ++r) {
+            if (bc_t[r] < there) {
+                const float* at = &red[cur][0][0][0][0] + threadIdx.x + 256 * r;
+                float s = at[0];
+#pragma unroll
+                for (int v = 1; v < WAVES; ++v) s += at[v * 2 * KT * NP];
+                *bc[r] = s;
+            }
+            bc[r] -= bc_tile;
         }
-        rn.move(-1);
-        lx.move(-J);
-        ldt.move(-J);
-        ldy.move(-J);
-        lz.move(-J);
         odx.move(-J);
         oddt.move(-J);
         odz.move(-J);
@@ -550,36 +626,47 @@ scan_bwd_kernel(ScanArgs a) {
     }
 }
 
-// dB, dC [t][b][g][n] from the channel tiles' partial sums, in tile order
+// dB, dC [t][b][g][n] from the channel tiles' partial sums, in tile order; a thread takes four states
 template <typename T>
 __global__ void __launch_bounds__(256)
 scan_fold_bc_kernel(const float* __restrict__ part, long long rows, int tiles, int np, int n, T* __restrict__ dB, T* __restrict__ dC) {
-    const long long total = rows * 2 * np;
+    const long long total = rows * 2 * np / 4;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
-        const int col = (int)(i % (2 * np)), k = col % np;
-        if (k >= n) continue;
-        float s = 0.f;
-        for (int t = 0; t < tiles; ++t) s += part[t * total + i];
-        (col < np ? dB : dC)[(i / (2 * np)) * n + k] = from_f<T>(s);
+        const int col = (int)(4 * i % (2 * np)), k = col % np;
+        const f32x4* p = reinterpret_cast<const f32x4*>(part) + i;
+        f32x4 s = p[0];
+#pragma unroll 4
+        for (int t = 1; t < tiles; ++t) s += p[t * total];
+        T* to = (col < np ? dB : dC) + 4 * i / (2 * np) * n + k;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+            if (k + c < n) to[c] = from_f<T>(s[c]);
     }
 }
-// dA [d][n], dD [d], dbias [d]: sums over the rows (batch elements), in row order, fp64
-__global__ void __launch_bounds__(256)
+// dA [d][n], dD [d], dbias [d]: sums over the rows (chunks, batch elements), fp64: 16 waves take every 16th row of 64 columns, then
+// wave order
+__global__ void __launch_bounds__(1024)
 scan_fold_params_kernel(const float* __restrict__ pa, const float* __restrict__ pd, int rows, int d, int np, int n, float* __restrict__ dA,
                         float* __restrict__ dD, float* __restrict__ db) {
-    const long long cols = (long long)d * (np + 2);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < cols; i += (long long)gridDim.x * 256) {
-        double s = 0.0;
-        if (i < (long long)d * np) {
-            if (i % np >= n) continue;
-            for (int r = 0; r < rows; ++r) s += (double)pa[(long long)r * d * np + i];
-            dA[(i / np) * n + i % np] = (float)s;
-        } else {
-            const long long j = i - (long long)d * np;
-            for (int r = 0; r < rows; ++r) s += (double)pd[(long long)r * d * 2 + j];
-            float* to = (j & 1) ? db : dD;
-            if (to) to[j >> 1] = (float)s;
-        }
+    __shared__ double red[16][64];
+    const int l = threadIdx.x & 63, g = threadIdx.x >> 6;
+    const long long i = (long long)blockIdx.x * 64 + l, na = (long long)d * np, all = na + 2ll * d;
+    double s = 0.0;
+    if (i < all) {
+        const float* p = i < na ? pa + i : pd + (i - na);
+        const long long row = i < na ? na : 2ll * d;
+#pragma unroll 8
+        for (int r = g; r < rows; r += 16) s += (double)p[r * row];
+    }
+    red[g][l] = s;
+    __syncthreads();
+    if (g != 0 || i >= all) return;
+    for (int k = 1; k < 16; ++k) s += red[k][l];
+    if (i < na) {
+        if (i % np < n) dA[(i / np) * n + i % np] = (float)s;
+    } else {
+        float* to = ((i - na) & 1) ? db : dD;
+        if (to) to[(i - na) >> 1] = (float)s;
     }
 }
 
@@ -614,6 +701,7 @@ scan_step_kernel(ScanArgs a) {
 
 int states_per_lane(int n) { return n <= 4 ? 1 : n <= 8 ? 2 : n <= 16 ? 4 : 8; }
 int tile_steps(int n) { return n <= 16 ? 16 : 8; }
+constexpr int SAVE_STEPS = Tile<1>::BACK;
 
 template <typename F> int scan_dispatch(int dtype, int n, F f) {
 #define JOVA_SCAN_NS(NS)                                                                  \
@@ -635,8 +723,8 @@ template <typename F> int scan_dispatch(int dtype, int n, F f) {
 int scan_check(const char* who, int dtype, int64_t steps, int64_t batch, int d, int groups, int n) {
     JOVA_CHECK_ARG(jova_dtype_ok(dtype), "%s: unknown dtype %d", who, dtype);
     JOVA_CHECK_ARG(steps >= 0 && batch >= 0 && d >= 1 && groups >= 1 && n >= 1 && d % groups == 0, "%s: bad shape", who);
-    if (n > 32 || batch > 65535) {
-        jova_set_error("%s: %d states (at most 32), %lld sequences (at most 65535)", who, n, (long long)batch);
+    if (n > 32 || batch > 65535 || steps > (1ll << 31) - 64) {
+        jova_set_error("%s: %d states (at most 32), %lld sequences (at most 65535), %lld steps (below 2^31)", who, n, (long long)batch, (long long)steps);
         return JOVA_ERR_LIMIT;
     }
     return JOVA_OK;
@@ -646,7 +734,7 @@ ScanArgs scan_args(const void* x, const void* dt, const float* A, const void* B,
                    const float* bias, int64_t steps, int64_t batch, int d, int groups, int n, const int64_t* st, int softplus,
                    const int32_t* lengths, const float* state0) {
     ScanArgs a = {};
-    a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.bias = bias; a.steps = steps; a.batch = (int)batch;
+    a.x = x; a.dt = dt; a.A = A; a.B = B; a.C = C; a.D = D; a.z = z; a.bias = bias; a.steps = (int)steps; a.batch = (int)batch;
     a.d = d; a.groups = groups; a.n = n; a.softplus = softplus; a.lengths = lengths; a.state0 = state0;
     a.x_t = st[0]; a.x_b = st[1]; a.dt_t = st[2]; a.dt_b = st[3]; a.z_t = st[4]; a.z_b = st[5];
     a.B_t = st[6]; a.B_b = st[7]; a.B_g = st[8]; a.C_t = st[9]; a.C_b = st[10]; a.C_g = st[11];
@@ -675,26 +763,26 @@ Plan bwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return s
 
 dim3 scan_grid(const ScanArgs& a, int z = 1) { return dim3((unsigned)channel_tiles(a.d, a.groups), (unsigned)a.batch, (unsigned)z); }
 
-// Lane's 32-bit offsets: 3 steps and a channel, in bytes
+// Lane's 32-bit offsets: a tile of 16 steps and a channel, in bytes
 bool lane_ok(const ScanArgs& a) {
-    const long long lim = (1ll << 29);
-    return 3 * a.x_t + a.d < lim && 3 * a.dt_t + a.d < lim && 3 * a.z_t + a.d < lim && 3 * a.dy_t + a.d < lim &&
-           3 * (long long)a.batch * a.d + a.d < lim && a.x_t >= 0 && a.dt_t >= 0 && a.z_t >= 0 && a.dy_t >= 0;
+    const long long lim = (1ll << 30) - a.d;
+    return 16 * a.x_t < lim && 16 * a.dt_t < lim && 16 * a.z_t < lim && 16 * a.dy_t < lim && 16ll * a.batch * a.d < lim &&
+           a.x_t >= 0 && a.dt_t >= 0 && a.z_t >= 0 && a.dy_t >= 0;
 }
 #define JOVA_SCAN_LANES(who)                                                                    \
     if (!lane_ok(a)) {                                                                          \
-        jova_set_error(who ": a step of more than 2^29 / 3 elements");                          \
+        jova_set_error(who ": a step of more than 2^26 elements");                          \
         return JOVA_ERR_LIMIT;                                                                  \
     }
 
 size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
+#undef pick
 }  // namespace
 
 extern "C" size_t jova_selective_scan_checkpoint_bytes(int64_t steps, int64_t batch, int d, int n_state) {
     if (steps <= 0 || batch <= 0 || d < 1 || n_state < 1 || n_state > 32) return 256;
-    const int kt = tile_steps(n_state);
-    return (size_t)((steps + kt - 1) / kt) * batch * d * 4 * states_per_lane(n_state) * 4;
+    return (size_t)((steps + SAVE_STEPS - 1) / SAVE_STEPS) * batch * d * 4 * states_per_lane(n_state) * 4;
 }
 
 extern "C" size_t jova_selective_scan_fwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state) {
@@ -715,7 +803,7 @@ extern "C" int jova_selective_scan_fwd(const void* x, const void* dt, const floa
                            lengths_or_null, state0_or_null);
     JOVA_SCAN_LANES("selective_scan_fwd")
     const Plan p = fwd_plan(steps, batch, d, groups, n_state);
-    a.y = y; a.state_out = state_out_or_null; a.ckpt = (float*)checkpoints_or_null; a.chunk = p.chunk;
+    a.y = y; a.state_out = state_out_or_null; a.ckpt = (float*)checkpoints_or_null; a.chunk = (int)p.chunk;
     a.carry = (float*)workspace;
     a.esum = (float*)((char*)workspace + align256((size_t)p.chunks * batch * d * 4 * states_per_lane(n_state) * 4));
     const hipStream_t s = (hipStream_t)stream;
@@ -772,7 +860,7 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
     const BwdSpace sp = bwd_space(steps, batch, d, groups, n_state, p.chunks);
     char* ws = (char*)workspace;
     a.part_bc = (float*)(ws + sp.bc); a.part_a = (float*)(ws + sp.a); a.part_d = (float*)(ws + sp.d);
-    a.carry = (float*)(ws + sp.carry); a.esum = (float*)(ws + sp.esum); a.chunk = p.chunk;
+    a.carry = (float*)(ws + sp.carry); a.esum = (float*)(ws + sp.esum); a.chunk = (int)p.chunk;
     a.dx = dx; a.ddt = ddt; a.dz = dz_or_null; a.dstate0 = dstate0_or_null;
     const hipStream_t s = (hipStream_t)stream;
     if (batch > 0) {
@@ -785,7 +873,7 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
             }
             hipLaunchKernelGGL((scan_bwd_kernel<T, NS>), scan_grid(a, p.chunks), dim3(256), 0, s, a);
             JOVA_CHECK_LAUNCH("selective_scan_bwd");
-            const long long rows = (long long)steps * batch * groups, total = rows * 2 * np;
+            const long long rows = (long long)steps * batch * groups, total = rows * 2 * np / 4;
             if (total) {
                 hipLaunchKernelGGL((scan_fold_bc_kernel<T>), dim3((unsigned)(total + 255 < 256ll * 4096 ? (total + 255) / 256 : 4096)), dim3(256), 0,
                                    s, a.part_bc, rows, tiles, np, n_state, (T*)dB, (T*)dC);
@@ -796,7 +884,7 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
         if (rc) return rc;
     }
     const long long cols = (long long)d * (np + 2);
-    hipLaunchKernelGGL(scan_fold_params_kernel, dim3((unsigned)((cols + 255) / 256)), dim3(256), 0, s, a.part_a, a.part_d,
+    hipLaunchKernelGGL(scan_fold_params_kernel, dim3((unsigned)((cols + 63) / 64)), dim3(1024), 0, s, a.part_a, a.part_d,
                        (int)(batch * p.chunks), d, np, n_state, dA, dD_or_null, dbias_or_null);
     JOVA_CHECK_LAUNCH("selective_scan_bwd (parameters)");
     return JOVA_OK;

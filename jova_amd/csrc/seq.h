@@ -33,20 +33,22 @@ constexpr float LN2_F = 0.6931471805599453f;
 __device__ __forceinline__ float sigmoid_f(float v) {
     return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-LOG2E_F * v));
 }
-// log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1], and log1p(e) = 2 atanh(s) with s = e / (2 + e) <= 1/3:
-// the series s + s^3/3 + .. + s^15/15 leaves s^17/17 * 2 < 1e-9, so small results keep their relative accuracy (a plain
-// log(1 + e) loses it: steps of 1e-3 are ordinary inputs of the scan).
+// log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| in (0, 1], and log1p(e) = 2 atanh(s) with s = e / (2 + e) <= 1/3, so small
+// results keep their relative accuracy (a plain log(1 + e) loses it: steps of 1e-3 are ordinary inputs of the scan).  atanh(s)/s
+// is a polynomial of degree 4 in s^2, fitted for the smallest largest relative error on [0, 1/9]: 8e-9, an eighth of fp32's.
 __device__ __forceinline__ float softplus_f(float v) {
     const float e = __builtin_amdgcn_exp2f(-LOG2E_F * fabsf(v));
     const float s = e * __builtin_amdgcn_rcpf(2.f + e), q = s * s;
-    float p = 1.f / 15.f;
-    p = fmaf(p, q, 1.f / 13.f);
-    p = fmaf(p, q, 1.f / 11.f);
-    p = fmaf(p, q, 1.f / 9.f);
-    p = fmaf(p, q, 1.f / 7.f);
-    p = fmaf(p, q, 1.f / 5.f);
-    p = fmaf(p, q, 1.f / 3.f);
+    float p = fmaf(0.14089167f, q, 0.13980301f);
+    p = fmaf(p, q, 0.20012455f);
+    p = fmaf(p, q, 0.33333158f);
     p = fmaf(p * q, s, s);
-    // fmaxf would drop a NaN
-    return (v > 0.f ? v : (v == v ? 0.f : v)) + 2.f * p;
+    return fmaf(2.f, p, v > 0.f ? v : 0.f);
+}
+
+// LDS accesses of a wave's lanes on either side stay on theirs (the hardware keeps a wave's LDS operations in order)
+__device__ __forceinline__ void wave_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+__device__ __forceinline__ void wave_order() {
+    wave_fence();
+    __builtin_amdgcn_wave_barrier();
 }
