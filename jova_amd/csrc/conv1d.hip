@@ -67,7 +67,7 @@ conv_fwd_kernel(ConvArgs a) {
     }
     T* y = (T*)a.y + b * (long long)a.d + c;
     const long long y_t = (long long)a.batch * a.d;
-    auto one = [&](const Pack<T, V>& in, long long t, bool live) {
+    auto one = [&](const Pack<T, V>& in, long long t) {
         Pack<T, V> out;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
@@ -78,7 +78,7 @@ conv_fwd_kernel(ConvArgs a) {
 #pragma unroll
             for (int k = 0; k < W; ++k) p = fmaf(w[v][k], win[k][v], p);
             if (a.silu) p *= sigmoid_f(p);
-            out.v[v] = from_f<T>(live ? p : 0.f);
+            out.v[v] = from_f<T>(p);
         }
         *(Pack<T, V>*)(y + t * y_t) = out;
     };
@@ -89,9 +89,10 @@ conv_fwd_kernel(ConvArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) in[u] = *(const Pack<T, V>*)(x + u * a.x_t);
 #pragma unroll
-        for (int u = 0; u < U; ++u) one(in[u], t + u, true);
+        for (int u = 0; u < U; ++u) one(in[u], t + u);
     }
-    for (; t < t1; ++t) one(conv_in<T, W, V>(a, t, b, c, len), t, t < len);
+    for (; t < min(t1, len); ++t) one(conv_in<T, W, V>(a, t, b, c, len), t);
+    for (; t < t1; ++t) *(Pack<T, V>*)(y + t * y_t) = none<T, V>();
     if (a.state_out && blockIdx.z == 0) {
 #pragma unroll
         for (int k = 0; k + 1 < W; ++k)
@@ -162,7 +163,7 @@ conv_bwd_kernel(ConvArgs a) {
             out.v[v] = from_f<T>(acc[0][v] + to_f(so.v[v]));
         }
         if (s >= lo && s < t1) {
-            if (s >= 0) *(Pack<T, V>*)(dx + s * dx_t) = (inner || s < len) ? out : none<T, V>();
+            if (s >= 0) *(Pack<T, V>*)(dx + s * dx_t) = out;
             else *(Pack<T, V>*)((T*)a.dstate + ((s + W - 1) * a.batch + b) * (long long)a.d + c) = out;
         }
     };
@@ -180,8 +181,9 @@ conv_bwd_kernel(ConvArgs a) {
 #pragma unroll
         for (int u = 0; u < U; ++u) one(in[u], gr[u], t + u, true, inner);
     }
-    for (; t < t1 + W - 1; ++t)
+    for (; t < min(t1, len) + W - 1; ++t)                // (behind the end: what is left of the last W - 1 gradients)
         one(conv_in<T, W, V>(a, t, b, c, len), t < len ? *(const Pack<T, V>*)(dy + t * a.dy_t + b * a.dy_b + c) : none<T, V>(), t, t < t1, false);
+    for (long long s = max(t0, len); s < t1; ++s) *(Pack<T, V>*)(dx + s * dx_t) = none<T, V>();
     float* part = a.part + ((long long)blockIdx.z * a.batch + b) * (W + 1) * a.d + c;
 #pragma unroll
     for (int v = 0; v < V; ++v) {

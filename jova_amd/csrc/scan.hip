@@ -57,12 +57,26 @@ struct Where {
     bool live;                                         // the channel exists
     int len;
 };
+// Sequences of a ragged batch start longest first (up to 256 of them: every workgroup ranks the lengths itself), so that a long one
+// does not begin when the others end.
+__device__ __forceinline__ int sequence_of(const ScanArgs& a, int slot) {
+    if (!a.lengths || a.batch > 256) return slot;
+    __shared__ int len[256], chosen;
+    const int t = threadIdx.x, mine = t < a.batch ? a.lengths[t] : 0;
+    len[t] = mine;
+    __syncthreads();
+    int rank = 0;
+    for (int k = 0; k < a.batch; ++k) rank += len[k] > mine || (len[k] == mine && k < t);
+    if (t < a.batch && rank == slot) chosen = t;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(chosen);
+}
 __device__ __forceinline__ Where where(const ScanArgs& a) {
     Where w;
     const int dg = a.d / a.groups, tiles = (dg + CH - 1) / CH;
     w.g = blockIdx.x / tiles;
     w.tile = blockIdx.x % tiles;
-    w.b = blockIdx.y;
+    w.b = sequence_of(a, blockIdx.y);
     w.q = threadIdx.x & 3;
     const int c = w.tile * CH + (threadIdx.x >> 2);
     w.live = c < dg;
