@@ -200,7 +200,8 @@ template <int NS> __device__ __forceinline__ void carry_in(const ScanArgs& a, co
         const Part<NS> p = *part_at<NS>(a.carry, a, w, c);
         const float e = a.esum[((long long)c * a.batch + w.b) * a.d + w.ch];
 #pragma unroll
-        for (int k = 0; k < NS; ++k) h[k] = fmaf(__builtin_amdgcn_exp2f(e * A2[k]), h[k], p.v[k]);
+        for (int k = 0; k < NS; ++k)                   // (nothing stays nothing, also where a growing state's factor overflows)
+            h[k] = h[k] == 0.f ? p.v[k] : fmaf(__builtin_amdgcn_exp2f(e * A2[k]), h[k], p.v[k]);
     }
 }
 template <typename F> __device__ __forceinline__ void four(F f) {

@@ -875,11 +875,15 @@ class EmbeddingFunction(torch.autograd.Function):
 
     @staticmethod
     def raise_if_bad():
-        """One device->host read, off the hot loop: IndexError if any lookup so far had an id outside the table."""
+        """One device->host read (a device), off the hot loop: IndexError if any lookup so far had an id outside the table."""
         f = EmbeddingFunction.bad_flag
         if f is not None and int(f.item()):
             f.zero_()
             raise IndexError("index out of range in self (fingerprint id outside the embedding table)")
+        for f in _TOKEN_FLAGS.values():
+            if int(f.item()):
+                f.zero_()
+                raise IndexError("index out of range in self (token id outside the embedding table)")
 
 
 class BlockAdjacency(object):
@@ -1204,12 +1208,16 @@ def embedding(idx, weight, scale=1.0, padding_idx=None):
     return _embedding_fwd(idx.to(torch.int64).contiguous(), weight, float(scale))
 
 
+_TOKEN_FLAGS = {}        # device -> int32 [1], set by embedding() where an id lies outside its table; kept (captured graphs write it)
+
+
 def _bad_flag(device):
-    f = EmbeddingFunction.bad_flag
-    if f is None or f.device != device:
+    f = _TOKEN_FLAGS.get(device)
+    if f is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("embedding: run it once on %s before capturing it into a graph (its error flag is made then)" % device)
-        f = EmbeddingFunction.bad_flag = torch.zeros(1, dtype=torch.int32, device=device)
+        f = _TOKEN_FLAGS[device] = torch.zeros(1, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()            # once: other streams use it from now on
     return f
 
 

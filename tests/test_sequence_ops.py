@@ -222,13 +222,13 @@ def test_embedding_gradient_adds_to_an_existing_grad_and_leaves_other_rows(devic
 def test_embedding_ids_outside_the_table(device):
     from jova_amd.nn import functional as F
     w = torch.randn(9, 4, device=device, requires_grad=True)
-    F.EmbeddingFunction.bad_flag = None
     out = F.embedding(torch.tensor([[0, 9], [-1, 8]], device=device), w)
     assert out.shape == (2, 2, 4) and torch.isnan(out[0, 1]).all() and torch.isnan(out[1, 0]).all() and torch.equal(out[1, 1], w[8])
     dw, = torch.autograd.grad(out, w, torch.ones_like(out))
     assert torch.equal(dw.sum(1).cpu(), torch.tensor([4., 0, 0, 0, 0, 0, 0, 0, 4.]))
     with pytest.raises(IndexError):
         F.EmbeddingFunction.raise_if_bad()
+    F.EmbeddingFunction.raise_if_bad()                               # (reported once)
 
 
 @pytest.mark.gpu
@@ -247,6 +247,25 @@ def test_embedding_one_hot_token_over_many_tiles(device):
     close(out, want, want.abs(), 2, "out")
     got, = torch.autograd.grad(out, wd, dout.to(device))
     close(got, dw, mag * (count[:, None].sqrt() + 4), 4, "dweight")     # (tile sums added up: far fewer than count roundings in a row)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [3, 600, 300000])
+def test_embedding_gradient_of_many_rows(device, vocab):
+    """300 001 rows: more than one round per sorting workgroup; one, two and three passes.  The rows are small integers, so every sum is
+    exact in fp32 and equals the float64 one."""
+    from jova_amd.nn import functional as F
+    g = gen(vocab)
+    n, d = 300001, 4
+    idx = (torch.rand(n, generator=g, dtype=torch.float64) ** 3 * vocab).long()
+    idx[::7] = -1                                                    # outside: no gradient
+    dout = torch.randint(-4, 5, (n, d), generator=g).float()
+    want = torch.zeros(vocab, d, dtype=torch.float64).index_add_(0, idx[idx >= 0], dout[idx >= 0].double())
+    w = torch.zeros(vocab, d, device=device, requires_grad=True)
+    got, = torch.autograd.grad(F.embedding(idx.to(device), w), w, dout.to(device))
+    assert torch.equal(got.double().cpu(), want)
+    with pytest.raises(IndexError):
+        F.EmbeddingFunction.raise_if_bad()
 
 
 # ------------------------------------------------------------------------------------------------ convolution (GPU)
@@ -320,6 +339,41 @@ def test_conv_strides_padding_garbage_and_pieces(device):
     for s in range(t):
         parts.append(F.causal_conv1d_step(full[s], st, pw.detach(), pb.detach(), "silu"))
     assert torch.equal(torch.stack(parts), whole) and torch.equal(st, end)
+
+
+@pytest.mark.gpu
+def test_conv_fp32_weights_on_16_bit_inputs_and_accumulated_gradients(device):
+    """Master weights in fp32 next to bf16 activations; a .grad that is there is added to; frozen parameters get none; misaligned rows."""
+    from jova_amd.nn import functional as F
+    g = gen(8)
+    t, b, d, width = 66, 2, 12, 3
+    wide = torch.randn(t, b, d + 1, generator=g).bfloat16()
+    w, bias, dy = torch.randn(d, width, generator=g), torch.randn(d, generator=g), torch.randn(t, b, d, generator=g).bfloat16()
+    x = wide[..., 1:]                                                # two bytes off every vector boundary
+    ref = R.conv(x, w, bias, True, None, None, dy)
+    mag = R.conv(x, w, bias, True, None, None, dy, mag=True)
+    xd = wide.to(device)[..., 1:]
+    pw, pb = w.to(device).requires_grad_(True), bias.to(device).requires_grad_(True)
+    pw.grad, pb.grad = torch.full_like(pw, 2.0), torch.full_like(pb, -3.0)
+    y = F.causal_conv1d(xd, pw, pb, "silu")
+    close(y, ref[0], 1.1 * mag[0], 20, "y")
+    y.backward(dy.to(device))
+    close(pw.grad, ref[3] + 2.0, mag[3] + 2.0, 22 + t * b, "dweight")
+    close(pb.grad, ref[4] - 3.0, mag[4] + 3.0, 22 + t * b, "dbias")
+    frozen = w.to(device)
+    pb.grad = None
+    y = F.causal_conv1d(xd, frozen, pb, "silu")
+    y.backward(dy.to(device))
+    assert frozen.grad is None
+    close(pb.grad, ref[4], mag[4], 22 + t * b, "dbias alone")
+    lx = xd.clone().requires_grad_(True)
+    y = F.causal_conv1d(lx, frozen, None, "silu")
+    y.backward(dy.to(device))
+    assert lx.grad.dtype == torch.bfloat16 and torch.isfinite(lx.grad).all()
+    with pytest.raises(RuntimeError, match="twice differentiable|once_differentiable|does not require grad|once"):
+        z = F.causal_conv1d(lx, frozen, None, "silu")
+        gx, = torch.autograd.grad(z.float().sum(), lx, create_graph=True)
+        gx.float().sum().backward()
 
 
 # ------------------------------------------------------------------------------------------------ scan (GPU)
@@ -470,6 +524,66 @@ def test_scan_long_sequence_and_extreme_time_steps(device):
     got = torch.autograd.grad((y, h), list(v.values()), (dy.to(device), dh.to(device)))
     for k, x in zip(v, got):
         close(x, ref[2][k], mag[2][k], 2 * c, "d" + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("batch,n", [(3, 16), (3, 20), (300, 4)])
+def test_scan_ragged_batches_over_several_chunks(device, batch, n):
+    """Sequences that end in different chunks of the split time axis (and more of them than a workgroup ranks): against runs of
+    each sequence by itself, cut to its length, whose time axis is split elsewhere or not at all."""
+    from jova_amd.nn import functional as F
+    g = gen(batch + n)
+    t, d = (700, 24) if batch == 3 else (40, 24)
+    a, dy, dh = scan_inputs(g, t, batch, d, n, 1, torch.float32)
+    lengths = torch.randint(0, t + 1, (batch,), generator=g)
+    lengths[:3] = torch.tensor([t, t // 5, 0])
+    keys = ("x", "dt", "A", "B", "C", "D", "z", "bias", "state")
+
+    def run(v, dy, dh, lens):
+        v = {k: x.to(device).requires_grad_(True) for k, x in v.items()}
+        y, h = F.selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], v["D"], v["z"], v["bias"], True, lens, v["state"], True)
+        gr = torch.autograd.grad((y, h), [v[k] for k in keys], (dy.to(device), dh.to(device)))
+        return y.detach(), h.detach(), dict(zip(keys, gr))
+    y, h, gr = run(a, dy, dh, lengths.to(device))
+    mag = R.scan(*(a[k] for k in keys[:8]), True, lengths, a["state"], dy, dh, mag=True) if batch == 3 else None
+    c = 4 * scan_c(t, n)
+    tot = {k: torch.zeros(a[k].shape, dtype=torch.float64) for k in ("A", "D", "bias")}
+    for i in (range(batch) if batch == 3 else (0, 1, 2, 150, 299)):
+        m = int(lengths[i])
+        one = {k: (x[:m, i:i + 1] if x.dim() >= 3 and k != "state" else x[i:i + 1] if k == "state" else x) for k, x in a.items()}
+        y1, h1, g1 = run(one, dy[:m, i:i + 1], dh[i:i + 1], None)
+        mi = R.scan(*(one[k] for k in keys[:8]), True, None, one["state"], dy[:m, i:i + 1], dh[i:i + 1], mag=True) if m else None
+        if m:
+            close(y[:m, i:i + 1], y1.double().cpu(), mi[0], c, "y")
+            for k in ("x", "dt", "z", "B", "C"):
+                close(gr[k][:m, i:i + 1], g1[k].double().cpu(), mi[2][k], 2 * c, "d" + k)
+            close(h[i:i + 1], h1.double().cpu(), mi[1], c, "state")
+            close(gr["state"][i:i + 1], g1["state"].double().cpu(), mi[2]["state"], 2 * c, "dstate")
+        else:
+            assert torch.equal(h[i], a["state"][i].to(device)) and torch.equal(gr["state"][i], dh[i].to(device))
+        assert float(y[m:, i].abs().sum()) == 0.0 and all(float(gr[k][m:, i].abs().sum()) == 0.0 for k in ("x", "dt", "z", "B", "C"))
+        for k in tot:
+            tot[k] += g1[k].double().cpu()
+    if batch == 3:
+        for k in tot:
+            close(gr[k], tot[k], mag[2][k], 2 * c + t * batch, "d" + k)
+
+
+@pytest.mark.gpu
+def test_scan_growing_states_and_silent_channels(device):
+    """A > 0 over a split time axis: a channel without input stays at zero although its factor over a chunk overflows."""
+    from jova_amd.nn import functional as F
+    t, d = 1200, 4
+    x = torch.zeros(t, 1, d, device=device)
+    x[:, :, 0] = 1e-3
+    dt = torch.full((t, 1, d), 0.5, device=device)
+    A = torch.full((d, 2), 0.9, device=device)
+    A[0] = -1.0
+    B = torch.ones(t, 1, 2, device=device)
+    y, h = F.selective_scan(x, dt, A, B, B, return_final_state=True)
+    assert float(y[..., 1:].abs().max()) == 0.0 and float(h[:, 1:].abs().max()) == 0.0
+    end = 0.5e-3 / (1 - math.exp(-0.5))                              # the geometric series' limit
+    assert abs(float(h[0, 0, 0]) - end) <= 1e-5 * end
 
 
 @pytest.mark.gpu
