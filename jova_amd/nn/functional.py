@@ -1136,6 +1136,14 @@ def _check_type(who, name, t, dtype, ref):
         raise RuntimeError("%s: %s is on %s, the input on %s" % (who, name, t.device, ref.device))
 
 
+def _all_like(dtype, dev, tensors):
+    """Whether every tensor that is given has this type and device (the fast way past _check_type, which names the culprit)."""
+    for t in tensors:
+        if t is not None and (not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.get_device() != dev):
+            return False
+    return True
+
+
 def _check_input(who, ref, dims):
     if not isinstance(ref, torch.Tensor) or ref.dtype not in _DTYPE_CODE:
         raise TypeError("%s takes float32, bfloat16 or float16 tensors, got %s" % (who, ref.dtype if torch.is_tensor(ref) else type(ref)))
@@ -1258,8 +1266,9 @@ def _conv_args(who, x, weight, bias, activation, dims):
         raise ValueError("%s: weight must be [%d, 2 .. 8], got %s" % (who, d, list(weight.shape) if torch.is_tensor(weight) else weight))
     if weight.dtype != x.dtype and weight.dtype != _F32:
         raise TypeError("%s: weight must be %s or float32, got %s" % (who, x.dtype, weight.dtype))
-    _check_type(who, "weight", weight, weight.dtype, x)
-    _check_type(who, "bias", bias, weight.dtype, x)
+    if not _all_like(weight.dtype, x.get_device(), (weight, bias)):
+        _check_type(who, "weight", weight, weight.dtype, x)
+        _check_type(who, "bias", bias, weight.dtype, x)
     _check_shape(who, "bias", bias, (d,))
     if activation is not None and activation != "silu":
         raise ValueError("%s: activation must be None or 'silu', got %r" % (who, activation))
@@ -1370,14 +1379,19 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, out_state=N
 def _scan_check(who, x, dt, A, B, C, D, z, dt_bias, dims):
     _check_input(who, x, dims)
     kind, shape, d = x.dtype, x.shape, x.shape[-1]
-    for name, t in (("dt", dt), ("B", B), ("C", C), ("z", z)):
-        _check_type(who, name, t, kind, x)
-    for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
-        _check_type(who, name, t, _F32, x)
+    dev = x.get_device()
+    if not _all_like(kind, dev, (dt, B, C, z)) or not _all_like(_F32, dev, (A, D, dt_bias)):
+        for name, t in (("dt", dt), ("B", B), ("C", C), ("z", z)):
+            _check_type(who, name, t, kind, x)
+        for name, t in (("A", A), ("D", D), ("dt_bias", dt_bias)):
+            _check_type(who, name, t, _F32, x)
+    if dt is None or B is None or C is None or A is None:
+        raise TypeError("%s: dt, A, B and C are needed" % who)
     if A.dim() != 2 or A.shape[0] != d or not 1 <= A.shape[1] <= 32:
         raise ValueError("%s: A must be [%d, 1 .. 32], got %s" % (who, d, list(A.shape)))
-    _check_shape(who, "dt", dt, shape)
-    _check_shape(who, "z", z, shape)
+    if dt.shape != shape or (z is not None and z.shape != shape):
+        _check_shape(who, "dt", dt, shape)
+        _check_shape(who, "z", z, shape)
     _check_shape(who, "D", D, (d,))
     _check_shape(who, "dt_bias", dt_bias, (d,))
     bs = B.shape
