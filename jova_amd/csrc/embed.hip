@@ -467,6 +467,8 @@ extern "C" int jova_token_embedding_bwd(const void* dout, int dtype, const int64
     JOVA_CHECK_ARG(jova_dtype_ok(dtype), "token_embedding_bwd: unknown dtype %d", dtype);
     JOVA_CHECK_ARG(n >= 0 && d >= 1 && vocab >= 1 && dweight && (n == 0 || (dout && idx && workspace)), "token_embedding_bwd: bad argument");
     JOVA_CHECK_ARG(n < (1ll << 31) && vocab < (1ll << 31) - 1, "token_embedding_bwd: at most 2^31 - 1 rows and tokens");
+    const int gw_max = gw_of(d);                       // (of one element a lane; a wider one takes fewer)
+    JOVA_CHECK_ARG((n + TILE - 1) / TILE * (gw_max <= 64 ? 256 : 4 * gw_max) < (1ll << 32), "token_embedding_bwd: too many rows of that width for one grid");
     hipStream_t s = (hipStream_t)stream;
     long long n16 = 0;
     int n_rest = 0;

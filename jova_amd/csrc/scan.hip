@@ -617,7 +617,7 @@ scan_bwd_kernel(ScanArgs a) {
                 float s = at[0];
 #pragma unroll
                 for (int v = 1; v < WAVES; ++v) s += at[v * 2 * KT * NP];
-                *bc[r] = s;
+                *bc[r] = bc_t[r] < now ? s : 0.f;      // (0 inf = NaN behind the end of a sequence whose state overflowed)
             }
             bc[r] -= bc_tile;
         }

@@ -9,6 +9,7 @@ returns ``None`` for that input; otherwise a zero tensor is allocated, filled an
 """
 import ctypes
 import math
+import weakref
 
 import numpy as np
 import torch
@@ -1186,6 +1187,22 @@ def _wants_grad(*tensors):
     return False
 
 
+_EAGER = weakref.WeakSet()         # the graphs that eager calls of the functions below have built and that are still alive
+
+
+def _note_leaves(ctx, *tensors):
+    """Refuses a forward pass captured into a hipGraph while an eager graph of the same leaves lives that was built on another
+    stream: its gradient accumulators stay on that stream, and the captured backward pass would draw it into the capture, which
+    ends the process."""
+    ctx.stream = torch._C._cuda_getCurrentRawStream(tensors[0].get_device())
+    ctx.leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
+    if not torch.cuda.is_current_stream_capturing():
+        _EAGER.add(ctx)
+    elif any(o.stream != ctx.stream and any(a is b for a in o.leaves for b in ctx.leaves) for o in list(_EAGER)):
+        raise RuntimeError("capturing a differentiable call while an eager graph of the same leaf tensors is alive: drop its "
+                           "results first, or build it on the capture's stream")
+
+
 def _workspace(n, like):
     return torch.empty(int(n), dtype=torch.uint8, device=like.device)
 
@@ -1240,6 +1257,7 @@ def _embedding_fwd(idx, weight, scale):
 class TokenEmbeddingFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, weight, idx, scale, pad):
+        _note_leaves(ctx, weight)
         idx = idx.to(torch.int64).contiguous()
         ctx.save_for_backward(idx)
         ctx.param, ctx.scale, ctx.pad = weight, scale, pad
@@ -1305,6 +1323,7 @@ def _conv_fwd(x, weight, bias, state, lengths, silu, want_state):
 class CausalConvFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, lengths, silu, want_state):
+        _note_leaves(ctx, x, weight, bias, state)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, state, lengths)
         ctx.params, ctx.silu = (weight, bias), silu
@@ -1373,6 +1392,7 @@ def causal_conv1d_step(x, state, weight, bias=None, activation=None, out_state=N
     y = torch.empty((n, d), dtype=x.dtype, device=x.device)
     _call_on(x, "jova_causal_conv_step", x.data_ptr(), x.stride(0), state.data_ptr(), out.data_ptr(), _DTYPE_CODE[x.dtype], n, d,
              w.shape[1], w.data_ptr(), _ptr(_c_opt(bias)), _DTYPE_CODE[w.dtype], silu, y.data_ptr())
+    torch.autograd.graph.increment_version(out)        # written behind autograd's back: a graph that saved it must notice
     return y
 
 
@@ -1449,6 +1469,7 @@ def _scan_fwd(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_stat
 class SelectiveScanFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state):
+        _note_leaves(ctx, x, dt, A, B, C, D, z, dt_bias, state)
         ctx.set_materialize_grads(False)
         y, h, ckpt = _scan_fwd(x, dt, A, B, C, D, z, dt_bias, state, lengths, softplus, want_state, True)
         ctx.save_for_backward(x, dt, A, B, C, D, z, dt_bias, lengths, ckpt)
@@ -1495,6 +1516,7 @@ def selective_scan_step(x, dt, A, B, C, state, D=None, z=None, dt_bias=None, dt_
     _call_on(x, "jova_selective_scan_step", x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(), C.data_ptr(), _ptr(D), _ptr(z),
              _ptr(dt_bias), _DTYPE_CODE[x.dtype], b, d, B.shape[1], A.shape[1], st, 1 if dt_softplus else 0, state.data_ptr(), out.data_ptr(),
              y.data_ptr())
+    torch.autograd.graph.increment_version(out)
     return y
 
 

@@ -171,6 +171,33 @@ def test_python_refusals_without_a_gpu():
     assert float(clip_grad_norm_([torch.nn.Parameter(w)], 1.0)) == 0.0                # no gradients: nothing to do
 
 
+def test_a_grid_too_large_and_a_capture_over_an_eager_graph_are_refused(monkeypatch):
+    from jova_amd import _lib
+    from jova_amd.nn import functional as F
+    p = ctypes.c_void_p(4096)
+    with pytest.raises(RuntimeError, match="one grid"):              # 2^29 rows of 8: 2^24 tiles of 256 threads
+        _lib.call("jova_token_embedding_bwd", p, 1, p, 2 ** 29, 8, 10, -1, 1.0, p, 0, p, None)
+
+    class Graph:                                                     # stands for the context of a differentiable call
+        pass
+    now = dict(stream=1, capturing=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: now["stream"], raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now["capturing"])
+    w, other, x = torch.ones(2, requires_grad=True), torch.ones(2, requires_grad=True), torch.ones(2)
+    eager = Graph()
+    F._note_leaves(eager, x, w, None)
+    assert [t is w for t in eager.leaves] == [True]
+    now.update(stream=2, capturing=True)
+    F._note_leaves(Graph(), x, other)                                # other leaves
+    with pytest.raises(RuntimeError, match="eager graph"):
+        F._note_leaves(Graph(), x, w)
+    now["stream"] = 1
+    F._note_leaves(Graph(), x, w)                                    # built on the capture's own stream
+    now["stream"] = 2
+    del eager
+    F._note_leaves(Graph(), x, w)
+
+
 # ------------------------------------------------------------------------------------------------ embedding (GPU)
 EMB = [(1, 1, 1), (3, 5, 7), (64, 10, 22), (2049, 300, 33), (5000, 9049, 22), (300, 70000, 8), (4096, 2, 130), (777, 40, 2056), (0, 6, 4)]
 
@@ -834,3 +861,43 @@ def test_other_stream_and_empty_shapes(device):
         assert y.shape == shape and torch.equal(h, h0)
         gh, gA = torch.autograd.grad(h.sum() + y.sum(), (h0, Al))
         assert torch.equal(gh, torch.ones_like(h0)) and float(gA.abs().max()) == 0.0
+
+
+@pytest.mark.gpu
+def test_scan_gradients_behind_the_end_of_an_overflowed_sequence(device):
+    """A state that has grown to infinity: its own gradients are not finite, the rows behind its end and the other sequence are."""
+    from jova_amd.nn import functional as F
+    t, d, n = 21, 4, 2
+    ones = torch.ones(t, 2, d, device=device)
+    x, dt = ones.clone(), ones * torch.tensor([40.0, 0.1], device=device)[:, None]
+    B = torch.ones(t, 2, n, device=device)
+    leaves = [v.clone().requires_grad_(True) for v in (x, dt, B, B)]
+    A = torch.ones(d, n, device=device)
+    y = F.selective_scan(leaves[0], leaves[1], A, leaves[2], leaves[3], lengths=torch.tensor([11, 13], device=device))
+    assert not bool(torch.isfinite(y[10, 0]).any()) and float(y[11:, 0].abs().max()) == 0.0
+    for g in torch.autograd.grad(y, leaves, torch.ones_like(y)):
+        assert float(g[11:, 0].abs().max()) == 0.0 and float(g[13:, 1].abs().max()) == 0.0
+        assert bool(torch.isfinite(g[:, 1]).all())
+
+
+@pytest.mark.gpu
+def test_a_state_moved_on_in_place_is_noticed_by_the_graph_that_saved_it(device):
+    from jova_amd.nn import functional as F
+    x, state = torch.randn(5, 2, 8, device=device), torch.randn(3, 2, 8, device=device)
+    w = torch.randn(8, 4, device=device, requires_grad=True)
+    y = F.causal_conv1d(x, w, initial_state=state)
+    with torch.no_grad():
+        F.causal_conv1d_step(x[0], state, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    h, version = torch.zeros(2, 8, 4, device=device), 0
+    with torch.no_grad():
+        B = torch.randn(2, 4, device=device)
+        for _ in range(2):
+            F.selective_scan_step(x[0], x[0], -torch.ones(8, 4, device=device), B, B, h)
+            assert h._version > version
+            version = h._version
+    with torch.inference_mode():
+        state = torch.zeros(3, 2, 8, device=device)
+        F.causal_conv1d_step(x[0], state, w)
+        assert torch.equal(state[2], x[0])
