@@ -7,6 +7,7 @@ Parameter gradients: the kernels *accumulate*.  If a parameter already has a ``.
 them as views of one flat buffer that it zeroes once per step), the kernels add straight into it and the Function
 returns ``None`` for that input; otherwise a zero tensor is allocated, filled and returned to autograd.
 """
+import array
 import ctypes
 import math
 import weakref
@@ -1524,25 +1525,27 @@ def grad_norm_and_clip(grads, max_norm, kind=2, norm_scale=1.0, out=None):
     """Global norm of a list of gradient tensors (kind 2, 1, or 0 for the largest magnitude) times norm_scale, and the tensors
     scaled by min(1, max_norm / (norm + 1e-6)) in place or into ``out`` -> the norm, a float32 device scalar (no host read).
     Contiguous tensors of one device, types may be mixed; an output has its tensor's type and element count."""
-    who, n = "grad clipping", len(grads)
+    who, n, T = "grad clipping", len(grads), torch.Tensor
     outs = grads if out is None else out
     if len(outs) != n:
         raise ValueError("%s: %d outputs for %d tensors" % (who, len(outs), n))
+    # (bound by the host on a few dozen tensors: map over the tensors' own methods and array.array take two thirds of the time of
+    # comprehensions and ctypes arrays)
+    types = [g.dtype for g in grads]
     try:
-        codes = [_DTYPE_CODE[g.dtype] for g in grads]
+        codes = array.array("i", map(_DTYPE_CODE.__getitem__, types))
     except KeyError as e:
         raise TypeError("%s takes float32, bfloat16 or float16 tensors, got %s" % (who, e)) from None
-    sizes = [g.numel() for g in grads]
-    devs = {g.get_device() for g in grads}
-    dense = all([g.is_contiguous() for g in grads])
-    gp = (ctypes.c_void_p * n)(*[g.data_ptr() for g in grads])
-    op = gp
+    sizes = array.array("q", map(T.numel, grads))
+    devs = set(map(T.get_device, grads))
+    dense = all(map(T.is_contiguous, grads))
+    gp = op = array.array("Q", map(T.data_ptr, grads))
     if outs is not grads:
-        if [o.numel() for o in outs] != sizes or [o.dtype for o in outs] != [g.dtype for g in grads]:
+        if array.array("q", map(T.numel, outs)) != sizes or [o.dtype for o in outs] != types:
             raise ValueError("%s: an output must have its tensor's type and element count" % who)
-        devs |= {o.get_device() for o in outs}
-        dense = dense and all([o.is_contiguous() for o in outs])
-        op = (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+        devs.update(map(T.get_device, outs))
+        dense = dense and all(map(T.is_contiguous, outs))
+        op = array.array("Q", map(T.data_ptr, outs))
     if not dense:
         raise ValueError("%s takes contiguous tensors" % who)
     if len(devs) != 1:
@@ -1550,6 +1553,6 @@ def grad_norm_and_clip(grads, max_norm, kind=2, norm_scale=1.0, out=None):
     _lib.require_gpu(grads[0])
     norm = torch.empty((), dtype=_F32, device=grads[0].device)
     ws = _workspace(_lib.lib().jova_clip_grads_workspace_bytes(n), norm)
-    _call_on(norm, "jova_clip_grads", n, gp, op, (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*codes), kind, float(norm_scale),
-             float(max_norm), norm.data_ptr(), ws.data_ptr())
+    _call_on(norm, "jova_clip_grads", n, *[a.buffer_info()[0] for a in (gp, op, sizes, codes)], kind, float(norm_scale), float(max_norm),
+             norm.data_ptr(), ws.data_ptr())
     return norm
