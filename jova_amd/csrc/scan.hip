@@ -8,6 +8,14 @@
 // Layout: four neighbouring lanes (a quad) share a channel and hold a quarter of its states each (NS of them, padded with
 // states that stay zero), so a wave covers 16 channels.  Time goes in tiles of KT steps; within four steps lane q of a quad
 // loads, and later stores, step 4j + q, and the quad passes scalars around with quad_perm, which costs nothing extra.
+// The states of a step live in registers and in nothing else; the backward pass starts every 8 steps from a saved state (8 bytes per
+// element of x at 16 states) and computes the states between once more.
+//
+// Bound by the vector ALUs, not by memory: per element and state the forward pass has exp (2 issue slots), e A, u B and two
+// multiply-adds, the backward pass about 17 operations, against 8 and 22 bytes per element with 16 states in 16 bits.  Packed fp32
+// operations are not used.  B and C come in through LDS, 16 (8) steps at once, two sides, the next tile's loads in flight meanwhile.
+// 2048 x 8 x 2048, 16 states, bf16: chunk states 110 us (99 % VALU busy), forward 175 (85-89 %), chunk adjoints 105, backward 447 (86 %).
+// 16384 x 1 x 4096: 500 us, 240 of them chunk states.  232 x 128 x 512 ragged fp32: forward 61, backward 149, folds 12 us.
 #include "seq.h"
 
 #include <type_traits>
@@ -15,10 +23,16 @@
 namespace {
 
 constexpr int WAVES = 4, CH = 16 * WAVES;              // channels of a workgroup
+// Workgroups to aim at when the time axis is cut (scan_plan).  Cutting costs a second pass over all chunks but one, too few
+// workgroups leave the SIMDs with one or two waves.  Forward target 256, 512, 768, 1024, 2048, 4096: 16384 x 1 x 4096 takes 978,
+// 616, 561, 534, 500, 514 us, 2048 x 8 x 2048 with its backward pass 798, 823, 783, 787, 783, 804; backward target 512, 768, 1536: 880, 783, 791
+// (three waves a SIMD are all its registers allow).
 constexpr int MAX_CHUNKS = 64, FWD_TARGET = 2048, BWD_TARGET = 768;
+// Steps of a chunk at least: with 64, 232 x 128 x 512 (1024 workgroups uncut) would be cut too: 241 against 209 us; 256: no difference.
+constexpr int LEAST_CHUNK = 128;
 // Steps of a tile: the forward passes take 16 (loads, address arithmetic and the barrier are shared by more steps), the backward pass
 // 8, whose states fit the registers of three waves a SIMD; states are saved every 8 steps.  (16 and two waves: 565 against
-// 450 us on 2048 x 8 x 2048; 32 states need twice the registers a step, so 8 in all passes.)
+// 447 us on 2048 x 8 x 2048; 32 states need twice the registers a step, so 8 in all passes.)
 template <int NS> struct Tile { static constexpr int KT = NS <= 4 ? 16 : 8, BACK = 8; };
 
 struct ScanArgs {
@@ -58,7 +72,8 @@ struct Where {
     int len;
 };
 // Sequences of a ragged batch start longest first (up to 256 of them: every workgroup ranks the lengths itself), so that a long one
-// does not begin when the others end.
+// does not begin when the others end (232 x 128 x 512 ragged, forward and backward: 263 -> 211 us together with skipping the
+// tiles behind the ends).
 __device__ __forceinline__ int sequence_of(const ScanArgs& a, int slot) {
     if (!a.lengths || a.batch > 256) return slot;
     __shared__ int len[256], chosen;
@@ -221,7 +236,8 @@ template <typename F> __device__ __forceinline__ void four_back(F f) {
 // compiler from making branches of them), without z its loads read x.
 #define pick(c) __builtin_unpredictable(c)
 
-// LOCAL: the chunk's own contribution to the state (from zero) and its sum of e, for carry_in
+// LOCAL: the chunk's own contribution to the state (from zero) and its sum of e, for carry_in.  In the main pass y's sum over n is
+// the lane's NS terms, then one exchange for four steps (quad_scatter_sum) that leaves every lane the step it stores.
 template <typename T, int NS, bool LOCAL>
 __global__ void __launch_bounds__(256)
 scan_fwd_kernel(ScanArgs a) {
@@ -443,6 +459,9 @@ template <int NS> struct Sums {
     }
 };
 
+// One tile: its states forward from the saved one, kept in registers with their factors exp(e A), then the adjoint backwards.  The
+// products for dB and dC are summed over the wave's channels (Sums), over the four waves through LDS and over the channel
+// tiles by scan_fold_bc_kernel, each in a fixed order; dA, dD, dbias stay in registers and leave one row per chunk and sequence.
 template <typename T, int NS>
 __global__ void __launch_bounds__(256, NS == 8 ? 1 : 3)
 scan_bwd_kernel(ScanArgs a) {
@@ -688,6 +707,8 @@ scan_fold_params_kernel(const float* __restrict__ pa, const float* __restrict__ 
 template <typename T> __device__ __forceinline__ float of_token(const void* p, long long s_b, const Where& w) {
     return p ? to_f(((const T*)p)[w.b * s_b + w.ch]) : 0.f;
 }
+// One token per sequence, same lanes; a lane reads its states before it writes them, so the state may be its own output.  Bound
+// by launch latency: 4.3 us for 4 x 2048 x 16 (1.3 MB).
 template <typename T, int NS>
 __global__ void __launch_bounds__(256)
 scan_step_kernel(ScanArgs a) {
@@ -773,8 +794,8 @@ Plan scan_plan(int64_t steps, int64_t batch, int d, int groups, int n, int targe
     if (p.chunk < kt) p.chunk = kt;
     return p;
 }
-Plan fwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, FWD_TARGET, 128); }
-Plan bwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, BWD_TARGET, 128); }
+Plan fwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, FWD_TARGET, LEAST_CHUNK); }
+Plan bwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, BWD_TARGET, LEAST_CHUNK); }
 
 dim3 scan_grid(const ScanArgs& a, int z = 1) { return dim3((unsigned)channel_tiles(a.d, a.groups), (unsigned)a.batch, (unsigned)z); }
 

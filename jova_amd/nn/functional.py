@@ -1188,7 +1188,7 @@ def _wants_grad(*tensors):
     return False
 
 
-_EAGER = weakref.WeakSet()         # the graphs that eager calls of the functions below have built and that are still alive
+_EAGER = []              # weak references to the graphs that eager calls of the functions below have built
 
 
 def _note_leaves(ctx, *tensors):
@@ -1198,8 +1198,12 @@ def _note_leaves(ctx, *tensors):
     ctx.stream = torch._C._cuda_getCurrentRawStream(tensors[0].get_device())
     ctx.leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
     if not torch.cuda.is_current_stream_capturing():
-        _EAGER.add(ctx)
-    elif any(o.stream != ctx.stream and any(a is b for a in o.leaves for b in ctx.leaves) for o in list(_EAGER)):
+        _EAGER.append(weakref.ref(ctx))
+        if len(_EAGER) & 1023 == 0:
+            _EAGER[:] = [r for r in _EAGER if r() is not None]
+        return
+    alive = [o for o in [r() for r in _EAGER] if o is not None]
+    if any(o.stream != ctx.stream and any(a is b for a in o.leaves for b in ctx.leaves) for o in alive):
         raise RuntimeError("capturing a differentiable call while an eager graph of the same leaf tensors is alive: drop its "
                            "results first, or build it on the capture's stream")
 
