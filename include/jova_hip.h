@@ -378,7 +378,7 @@ enum { JOVA_F32 = 0, JOVA_BF16 = 1, JOVA_F16 = 2 };
  * Backward: dweight[v][:] = scale * sum over { r : idx[r] = v } of dout[r][:] in ascending r, summed in fp32 and rounded
  * once (accumulate = 0: every row of dweight is written, rows without a token as zeros; 1: added to what is there, untouched
  * rows stay).  Rows whose id is padding_idx (-1: none) or outside [0, vocab) add nothing.  No float atomics: the same bits on every call.
- * n, vocab < 2^31; dweight 16-byte aligned.  workspace (16-byte aligned): the bytes that the function names. */
+ * n, vocab < 2^31 (and n / 32 workgroups within one grid of 2^32 threads); dweight 16-byte aligned.  workspace (16-byte aligned): the bytes that the function names. */
 int jova_token_embedding_fwd(const void* weight, int dtype, const int64_t* idx, int64_t n, int d, int64_t vocab, float scale,
                              void* out, int* bad_flag, void* stream);
 size_t jova_token_embedding_bwd_workspace_bytes(int64_t n, int d, int64_t vocab);
@@ -389,7 +389,7 @@ int jova_token_embedding_bwd(const void* dout, int dtype, const int64_t* idx, in
  * weight [d, width], width 2 .. 8.  state [width-1, batch, d] (optional, x's type) = the inputs in front of x (zeros without it);
  * state_out (optional) receives the last width-1 inputs.  Backward: dweight / dbias are written (accumulate = 0) or added to;
  * dstate_out (optional) = gradient of state_out, dstate (optional) receives that of state.  step: one token a sequence,
- * x [batch, d] with row stride x_b; state_out may be state (updated in place). */
+ * x [batch, d] with row stride x_b; state_out may be state (updated in place).  At most 65535 sequences of 65535 * 64 steps. */
 int jova_causal_conv_fwd(const void* x, int64_t x_t, int64_t x_b, int dtype, int64_t steps, int64_t batch, int d, int width,
                          const void* weight, const void* bias_or_null, int weight_dtype, int silu,
                          const int32_t* lengths_or_null, const void* state_or_null, void* y, void* state_out_or_null,
@@ -408,7 +408,8 @@ int jova_causal_conv_step(const void* x, int64_t x_b, const void* state, void* s
  * x, dt, z, dy [steps, batch, d]; B, C [steps, batch, groups, n_state] (the d / groups channels of a group share them);
  * A [d, n_state], D, dt_bias [d] and the states [batch, d, n_state] are fp32; n_state <= 32.  strides: HOST array of 12 (elements):
  * time, batch of x, dt, z; time, batch, group of B, C.  state0 (optional) = h in front of the first step, state_out (optional)
- * = h behind the last.  checkpoints (optional, jova_selective_scan_checkpoint_bytes): states the forward leaves for the backward.
+ * = h behind the last.  checkpoints (optional, jova_selective_scan_checkpoint_bytes): states the forward leaves for the backward,
+ * one every 8 steps (n_state rounded up to 4, 8, 16, 32).  At most 65535 sequences, a step of at most 2^26 elements (strides too).
  * Backward: all gradients are written; dz with z, dD / dbias / dstate0 optional; dB, dC are sums over the group's channels.
  * step: one token a sequence (x [batch, d], B [batch, groups, n_state]; the time strides are ignored); state_out may be state. */
 size_t jova_selective_scan_checkpoint_bytes(int64_t steps, int64_t batch, int d, int n_state);

@@ -14,8 +14,9 @@
 // Bound by the vector ALUs, not by memory: per element and state the forward pass has exp (2 issue slots), e A, u B and two
 // multiply-adds, the backward pass about 17 operations, against 8 and 22 bytes per element with 16 states in 16 bits.  Packed fp32
 // operations are not used.  B and C come in through LDS, 16 (8) steps at once, two sides, the next tile's loads in flight meanwhile.
-// 2048 x 8 x 2048, 16 states, bf16: chunk states 110 us (99 % VALU busy), forward 175 (85-89 %), chunk adjoints 105, backward 447 (86 %).
-// 16384 x 1 x 4096: 500 us, 240 of them chunk states.  232 x 128 x 512 ragged fp32: forward 61, backward 149, folds 12 us.
+// 2048 x 8 x 2048, 16 states, bf16: chunk states 110 us (vector ALUs busy 92 %), forward 175 (90 %), chunk adjoints 105 (78 %), backward
+// 447 (86 %).
+// 16384 x 1 x 4096: 500 us, 240 of them chunk states (97 and 96 %).  232 x 128 x 512 ragged fp32: forward 61, backward 149, folds 12 us.
 #include "seq.h"
 
 #include <type_traits>
