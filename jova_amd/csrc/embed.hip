@@ -5,7 +5,8 @@
 // first sorted by token (stable, so the rows of one token stay in ascending order), then every token's run is summed in
 // that order in fp32 and rounded once: the same bits on every call.
 // Bound by memory (rows in, rows out, dW written whole) on long batches, by launches and the host on short ones.  65536 rows of
-// 2048 bf16, 131072 tokens: 303 us for 1.34 GB = 4.4 TB/s: lookup 86, sort with the zeros of dW 85, reduce 115, join 21.
+// 2048 bf16, 131072 tokens: 263 us for 1.34 GB = 5.1 TB/s (with cached accesses 297): lookup 84, sort with the zeros of dW 82, reduce
+// 72, join 15.
 // 119680 rows of 22 floats, 9049 tokens: 7 + 27 + 9 + 6 us on the card, 100 us a call (the autograd engine's thread and seven launches).
 #include "seq.h"
 
@@ -218,10 +219,24 @@ token_sort_small_kernel(SortArgs a, int passes, uint2* buf0, uint2* buf1) {
 }
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack { T v[VEC]; };
+template <int BYTES> struct Bits;
+template <> struct Bits<2> { typedef unsigned short type; };
+template <> struct Bits<4> { typedef unsigned type; };
+template <> struct Bits<8> { typedef unsigned long long type; };
+template <> struct Bits<16> { typedef f32x4 type; };
+// what is read or written once, past the cache
+template <typename P> __device__ __forceinline__ P load_once(const P* p) {
+    return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const typename Bits<sizeof(P)>::type*>(p)));
+}
+template <typename P> __device__ __forceinline__ void store_once(P* p, const P& v) {
+    typedef typename Bits<sizeof(P)>::type B;
+    __builtin_nontemporal_store(__builtin_bit_cast(B, v), reinterpret_cast<B*>(p));
+}
 
 // Flat over the output's 16-byte pieces (fewer bytes where the rows or addresses do not divide), so short rows fill the lanes too.
-// I: the index type that holds n * dv (64-bit divisions cost more than the row's copy).  65536 x 2048 bf16: 86 us for 0.54 GB, 6.2 TB/s
-// with the hot rows from the cache.
+// I: the index type that holds n * dv (64-bit divisions cost more than the row's copy).  The output goes past the cache, which then holds
+// more of the table's rows: 65536 x 2048 bf16 84 us for 0.54 GB, 6.4 TB/s with the hot rows from the cache; the whole call with its gradient
+// 264 us, with cached stores 276.
 template <typename T, int VEC, typename I>
 __global__ void __launch_bounds__(256)
 token_fwd_kernel(const T* __restrict__ w, const long long* __restrict__ idx, long long n, int dv, long long vocab, float scale,
@@ -249,7 +264,7 @@ token_fwd_kernel(const T* __restrict__ w, const long long* __restrict__ idx, lon
             if (e >= total) continue;
 #pragma unroll
             for (int j = 0; j < VEC; ++j) p[u].v[j] = from_f<T>(ok[u] ? to_f(p[u].v[j]) * scale : __int_as_float(0x7fc00000));
-            reinterpret_cast<Pack<T, VEC>*>(out)[e] = p[u];
+            store_once(reinterpret_cast<Pack<T, VEC>*>(out) + e, p[u]);
         }
     }
 }
@@ -267,13 +282,17 @@ __device__ __forceinline__ void write_row(T* dw, long long at, const float* acc,
 }
 
 // Entries of a tile: few give more rows that cross a border (16: 337 us for the whole call of 65536 x 2048 bf16, 32: 303, 64:
-// 299), many leave short rows with too few workgroups (22 floats a row: 3740 tiles of 32 on 16 lanes are 234 workgroups).
+// 299, with 8 rows requested ahead), many leave short rows with too few workgroups (22 floats a row: 3740 tiles of 32 on 16 lanes are 234 workgroups).
 constexpr int TILE = 32;
-template <typename T, int VEC>
+// Rows of this many 16-byte pieces (2 KB) and more are read past the cache, two ahead (more waves a SIMD); shorter ones share lines
+// with each other and are latency-bound: through the cache, eight ahead.  Gradient of 65536 rows, long against short form: 1 KB
+// 53 .. 56 against 53 us, 2 KB 71 against 73, 4 KB 111 against 122; 88-byte rows (119680 of them, the kernel alone) 16 against 9.
+constexpr int LONG_ROW = 128;
+template <typename T, int VEC, bool LONG>
 __global__ void __launch_bounds__(256)
 token_reduce_kernel(const uint2* __restrict__ order, const T* __restrict__ dout, long long n, int dv, unsigned vocab, int gw, float scale,
                     int accumulate, T* __restrict__ dw, float* __restrict__ head, float* __restrict__ tail) {
-    constexpr int U = 8;                               // rows requested before the first of them is added
+    constexpr int U = LONG ? 2 : 8;                    // rows requested while as many are added
     const int per = 256 / gw, g = threadIdx.x / gw;
     const long long t = (long long)blockIdx.x * per + g, e0 = t * TILE;
     const int c = blockIdx.y * 256 + threadIdx.x % gw;
@@ -286,6 +305,7 @@ token_reduce_kernel(const uint2* __restrict__ order, const T* __restrict__ dout,
     if (e0 >= n || c >= dv) return;
     const uint2* it = lds[g] + 1;
     const Pack<T, VEC>* rows = reinterpret_cast<const Pack<T, VEC>*>(dout) + c;
+    auto row_at = [&](unsigned r) { return LONG ? load_once(rows + (long long)r * dv) : rows[(long long)r * dv]; };
     float acc[VEC];
     unsigned cur = it[0].x;
     bool open = cur == it[-1].x;                       // the run began in an earlier tile
@@ -294,14 +314,14 @@ token_reduce_kernel(const uint2* __restrict__ order, const T* __restrict__ dout,
     Pack<T, VEC> p[U], ahead[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-        if (it[u].x < vocab) ahead[u] = rows[(long long)it[u].y * dv];
+        if (it[u].x < vocab) ahead[u] = row_at(it[u].y);
     for (int e = 0; e < TILE; e += U) {
 #pragma unroll
         for (int u = 0; u < U; ++u) p[u] = ahead[u];
         if (e + U < TILE)                              // in front of this batch's stores: a load behind a store waits for it
 #pragma unroll
             for (int u = 0; u < U; ++u)
-                if (it[e + U + u].x < vocab) ahead[u] = rows[(long long)it[e + U + u].y * dv];
+                if (it[e + U + u].x < vocab) ahead[u] = row_at(it[e + U + u].y);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const unsigned key = it[e + u].x;
@@ -431,8 +451,13 @@ int reduce_launch(const uint2* order, const void* dout, int64_t n, int d, int64_
     const int dv = d / VEC, gw = gw_of(dv), per = 256 / gw;
     const long long tiles = (n + TILE - 1) / TILE;
     const unsigned cols = (unsigned)((dv + 255) / 256);
-    hipLaunchKernelGGL((token_reduce_kernel<T, VEC>), dim3((unsigned)((tiles + per - 1) / per), cols), dim3(256), 0, s, order, (const T*)dout,
-                       (long long)n, dv, (unsigned)vocab, gw, scale, accumulate, (T*)dw, head, tail);
+    const dim3 grid((unsigned)((tiles + per - 1) / per), cols);
+    if (VEC * sizeof(T) == 16 && dv >= LONG_ROW)
+        hipLaunchKernelGGL((token_reduce_kernel<T, VEC, VEC * sizeof(T) == 16>), grid, dim3(256), 0, s, order, (const T*)dout, (long long)n, dv,
+                           (unsigned)vocab, gw, scale, accumulate, (T*)dw, head, tail);
+    else
+        hipLaunchKernelGGL((token_reduce_kernel<T, VEC, false>), grid, dim3(256), 0, s, order, (const T*)dout, (long long)n, dv, (unsigned)vocab,
+                           gw, scale, accumulate, (T*)dw, head, tail);
     JOVA_CHECK_LAUNCH("token_embedding_bwd (reduce)");
     if (tiles > 1) {
         const int threads = gw <= 64 ? 256 : 4 * gw;

@@ -14,7 +14,7 @@
 // Bound by the vector ALUs, not by memory: per element and state the forward pass has exp (2 issue slots), e A, u B and two
 // multiply-adds, the backward pass about 17 operations, against 8 and 22 bytes per element with 16 states in 16 bits.  Packed fp32
 // operations are not used.  B and C come in through LDS, 16 (8) steps at once, two sides, the next tile's loads in flight meanwhile.
-// 2048 x 8 x 2048, 16 states, bf16: chunk states 110 us (vector ALUs busy 92 %), forward 175 (90 %), chunk adjoints 105 (78 %), backward
+// 2048 x 8 x 2048, 16 states, bf16: chunk states 110 us (vector ALUs busy 92 %), forward 175 (90 %), chunk adjoints 92 (92 %), backward
 // 447 (86 %).
 // 16384 x 1 x 4096: 500 us, 240 of them chunk states (97 and 96 %).  232 x 128 x 512 ragged fp32: forward 61, backward 149, folds 12 us.
 #include "seq.h"
@@ -42,11 +42,12 @@ struct ScanArgs {
     void *y, *dx, *ddt, *dz;
     float *state_out, *dstate0;
     float* ckpt;                                       // [tiles][batch][d][4 NS]: the state in front of every tile
-    float *carry, *esum;                               // [chunks][batch][d][4 NS] and [chunks][batch][d]: carry_in
+    float *carry, *esum;                               // [chunks or pieces][batch][d][4 NS] and [..][batch][d]: carry_in
     float *part_bc, *part_a, *part_d;                  // partial sums of dB | dC, dA, dD | dbias
     const int* lengths;
     long long x_t, x_b, dt_t, dt_b, z_t, z_b, B_t, B_b, B_g, C_t, C_b, C_g, dy_t, dy_b;
     int steps, chunk;                                  // steps of a chunk (blockIdx.z), a multiple of KT
+    int piece, pieces;                                 // of the adjoint pass: steps of a piece of a chunk, pieces of a chunk
     int batch, d, groups, n, softplus;
 };
 
@@ -348,7 +349,8 @@ scan_fwd_kernel(ScanArgs a) {
     }
 }
 
-// The adjoint that a chunk hands to the one in front of it, from zero: q <- exp(e A) (q + C g), steps descending
+// The adjoint that a piece of a chunk hands to what is in front of it, from zero: q <- exp(e A) (q + C g), steps descending.  Its
+// registers allow more waves than the backward pass, whose chunks are cut into pieces for it (bwd_plan).
 template <typename T, int NS>
 __global__ void __launch_bounds__(256)
 scan_adjoint_kernel(ScanArgs a) {
@@ -356,8 +358,9 @@ scan_adjoint_kernel(ScanArgs a) {
     __shared__ __align__(16) float rows[2][2 * KT * NP];
     const Where w = where(a);
     const bool softplus = a.softplus, gate = a.z != nullptr;
-    const int chunk = blockIdx.z + 1;                  // nothing is in front of chunk 0
-    const int first = chunk * a.chunk, end = min(min(a.steps, first + a.chunk), max(first, w.len));
+    const int chunk = 1 + blockIdx.z / a.pieces, row = blockIdx.z + a.pieces;          // nothing is in front of chunk 0
+    const int first = chunk * a.chunk + blockIdx.z % a.pieces * a.piece;
+    const int end = min(min(a.steps, min(first + a.piece, (chunk + 1) * a.chunk)), max(first, w.len));
     const int top = end > first ? first + ((end - first - 1) / KT) * KT : first - KT;
     float A2[NS], q[NS], es = 0.f;
     load_A2<NS>(a, w, A2);
@@ -420,8 +423,8 @@ scan_adjoint_kernel(ScanArgs a) {
     Part<NS> p;
 #pragma unroll
     for (int k = 0; k < NS; ++k) p.v[k] = q[k];
-    *part_at<NS>(a.carry, a, w, chunk) = p;
-    if (w.q == 0) a.esum[((long long)chunk * a.batch + w.b) * a.d + w.ch] = es;
+    *part_at<NS>(a.carry, a, w, row) = p;
+    if (w.q == 0) a.esum[((long long)row * a.batch + w.b) * a.d + w.ch] = es;
 }
 
 // Sums over the wave's 16 channels of v[2][4][NS] (dB | dC, step, state), through the wave's own piece of LDS: written as
@@ -478,7 +481,7 @@ scan_bwd_kernel(ScanArgs a) {
     float A2[NS], q[NS], dA[NS], dD = 0.f, db = 0.f;
     load_A2<NS>(a, w, A2);
     load_state<NS>(a.dstate_out, a, w, q);
-    carry_in<NS>(a, w, A2, (int)gridDim.z - 1, (int)blockIdx.z, -1, q);
+    carry_in<NS>(a, w, A2, (int)gridDim.z * a.pieces - 1, ((int)blockIdx.z + 1) * a.pieces - 1, -1, q);
 #pragma unroll
     for (int k = 0; k < NS; ++k) dA[k] = 0.f;
     const float Dv = a.D ? a.D[w.ch] : 0.f, bias = a.bias ? a.bias[w.ch] : 0.f;
@@ -760,8 +763,8 @@ template <typename F> int scan_dispatch(int dtype, int n, F f) {
 int scan_check(const char* who, int dtype, int64_t steps, int64_t batch, int d, int groups, int n) {
     JOVA_CHECK_ARG(jova_dtype_ok(dtype), "%s: unknown dtype %d", who, dtype);
     JOVA_CHECK_ARG(steps >= 0 && batch >= 0 && d >= 1 && groups >= 1 && n >= 1 && d % groups == 0, "%s: bad shape", who);
-    if (n > 32 || batch > 65535 || steps > (1ll << 31) - 64) {
-        jova_set_error("%s: %d states (at most 32), %lld sequences (at most 65535), %lld steps (below 2^31)", who, n, (long long)batch, (long long)steps);
+    if (n > 32 || batch > 65535 || steps > (1ll << 31) - (1 << 16)) {           // (a chunk's end, rounded up to tiles, is an int too)
+        jova_set_error("%s: %d states (at most 32), %lld sequences (at most 65535), %lld steps (below 2^31 - 2^16)", who, n, (long long)batch, (long long)steps);
         return JOVA_ERR_LIMIT;
     }
     return JOVA_OK;
@@ -796,7 +799,19 @@ Plan scan_plan(int64_t steps, int64_t batch, int d, int groups, int n, int targe
     return p;
 }
 Plan fwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, FWD_TARGET, LEAST_CHUNK); }
-Plan bwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) { return scan_plan(steps, batch, d, groups, n, BWD_TARGET, LEAST_CHUNK); }
+struct BwdPlan : Plan { int pieces; long long piece; };
+BwdPlan bwd_plan(int64_t steps, int64_t batch, int d, int groups, int n) {
+    BwdPlan p = {scan_plan(steps, batch, d, groups, n, BWD_TARGET, LEAST_CHUNK), 1, 0};
+    p.piece = p.chunk;
+    if (p.chunks > 1) {
+        const long long kt = tile_steps(n), wgs = (long long)channel_tiles(d, groups) * batch * (p.chunks - 1);
+        long long c = FWD_TARGET / wgs;
+        if (c > p.chunk / LEAST_CHUNK) c = p.chunk / LEAST_CHUNK;
+        if (c > 1) p.piece = ((p.chunk + c - 1) / c + kt - 1) / kt * kt;
+        p.pieces = (int)((p.chunk + p.piece - 1) / p.piece);
+    }
+    return p;
+}
 
 dim3 scan_grid(const ScanArgs& a, int z = 1) { return dim3((unsigned)channel_tiles(a.d, a.groups), (unsigned)a.batch, (unsigned)z); }
 
@@ -859,22 +874,22 @@ extern "C" int jova_selective_scan_fwd(const void* x, const void* dt, const floa
 
 namespace {
 struct BwdSpace { size_t bc, a, d, carry, esum, all; };
-BwdSpace bwd_space(int64_t steps, int64_t batch, int d, int groups, int n, int chunks) {
-    const size_t np = 4 * states_per_lane(n), rows = (size_t)chunks * batch * d, tiles = (d / groups + CH - 1) / CH;
+BwdSpace bwd_space(int64_t steps, int64_t batch, int d, int groups, int n, const BwdPlan& p) {
+    const size_t np = 4 * states_per_lane(n), rows = (size_t)p.chunks * batch * d, tiles = (d / groups + CH - 1) / CH;
     BwdSpace s;
     s.bc = 0;
     s.a = s.bc + align256(tiles * steps * batch * groups * 2 * np * 4);
     s.d = s.a + align256(rows * np * 4);
     s.carry = s.d + align256(rows * 8);
-    s.esum = s.carry + align256(rows * np * 4);
-    s.all = s.esum + align256(rows * 4);
+    s.esum = s.carry + align256(rows * p.pieces * np * 4);
+    s.all = s.esum + align256(rows * p.pieces * 4);
     return s;
 }
 }  // namespace
 
 extern "C" size_t jova_selective_scan_bwd_workspace_bytes(int64_t steps, int64_t batch, int d, int groups, int n_state) {
     if (steps < 0 || batch <= 0 || d < 1 || groups < 1 || n_state < 1 || n_state > 32) return 256;
-    return bwd_space(steps, batch, d, groups, n_state, bwd_plan(steps, batch, d, groups, n_state).chunks).all;
+    return bwd_space(steps, batch, d, groups, n_state, bwd_plan(steps, batch, d, groups, n_state)).all;
 }
 
 extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const float* A, const void* B, const void* C,
@@ -893,11 +908,12 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
     a.dy = dy; a.dy_t = dy_t; a.dy_b = dy_b; a.dstate_out = dstate_out_or_null; a.ckpt = (float*)checkpoints;
     JOVA_SCAN_LANES("selective_scan_bwd")
     const int np = 4 * states_per_lane(n_state), tiles = (d / groups + CH - 1) / CH;
-    const Plan p = bwd_plan(steps, batch, d, groups, n_state);
-    const BwdSpace sp = bwd_space(steps, batch, d, groups, n_state, p.chunks);
+    const BwdPlan p = bwd_plan(steps, batch, d, groups, n_state);
+    const BwdSpace sp = bwd_space(steps, batch, d, groups, n_state, p);
     char* ws = (char*)workspace;
     a.part_bc = (float*)(ws + sp.bc); a.part_a = (float*)(ws + sp.a); a.part_d = (float*)(ws + sp.d);
     a.carry = (float*)(ws + sp.carry); a.esum = (float*)(ws + sp.esum); a.chunk = (int)p.chunk;
+    a.piece = (int)p.piece; a.pieces = p.pieces;
     a.dx = dx; a.ddt = ddt; a.dz = dz_or_null; a.dstate0 = dstate0_or_null;
     const hipStream_t s = (hipStream_t)stream;
     if (batch > 0) {
@@ -905,7 +921,7 @@ extern "C" int jova_selective_scan_bwd(const void* x, const void* dt, const floa
             typedef decltype(t) T;
             constexpr int NS = decltype(k)::value;
             if (p.chunks > 1) {
-                hipLaunchKernelGGL((scan_adjoint_kernel<T, NS>), scan_grid(a, p.chunks - 1), dim3(256), 0, s, a);
+                hipLaunchKernelGGL((scan_adjoint_kernel<T, NS>), scan_grid(a, (p.chunks - 1) * p.pieces), dim3(256), 0, s, a);
                 JOVA_CHECK_LAUNCH("selective_scan_bwd (chunks)");
             }
             hipLaunchKernelGGL((scan_bwd_kernel<T, NS>), scan_grid(a, p.chunks), dim3(256), 0, s, a);

@@ -901,3 +901,23 @@ def test_a_state_moved_on_in_place_is_noticed_by_the_graph_that_saved_it(device)
         state = torch.zeros(3, 2, 8, device=device)
         F.causal_conv1d_step(x[0], state, w)
         assert torch.equal(state[2], x[0])
+
+
+@pytest.mark.gpu
+def test_scan_backward_whose_chunks_are_cut_into_pieces(device):
+    """So many sequences that the time axis is cut into two chunks only, and the adjoint pass over the second into pieces."""
+    from jova_amd.nn import functional as F
+    g, t, b, d, n = gen(81), 620, 300, 2, 3
+    a, dy, dh = scan_inputs(g, t, b, d, n, 1, torch.float32)
+    lengths = torch.randint(0, t + 1, (b,), generator=g)
+    lengths[:4] = torch.tensor([t, t - 1, 330, 0])
+    keys = ("x", "dt", "A", "B", "C", "D", "z", "bias", "state")
+    v = {k: x.to(device).requires_grad_(True) for k, x in a.items()}
+    y, h = F.selective_scan(v["x"], v["dt"], v["A"], v["B"], v["C"], v["D"], v["z"], v["bias"], True, lengths.to(device), v["state"], True)
+    got = dict(zip(keys, torch.autograd.grad((y, h), [v[k] for k in keys], (dy.to(device), dh.to(device)))))
+    want, mag = (R.scan(*(a[k] for k in keys[:8]), True, lengths, a["state"], dy, dh, mag=m) for m in (False, True))
+    c = scan_c(t, n)
+    close(y, want[0], mag[0], c, "y")
+    close(h, want[1], mag[1], c, "state")
+    for k in keys:                                                   # (the parameters' sums run over the batch too)
+        close(got[k], want[2][k], mag[2][k], 2 * c + (t * b if k in ("A", "D", "bias") else 0), "d" + k)
