@@ -388,7 +388,7 @@ int jova_token_embedding_bwd(const void* dout, int dtype, const int64_t* idx, in
 /* Causal depthwise convolution: p[t] = bias + sum_{k<width} weight[:, k] x[t - width + 1 + k], y = p or p * sigmoid(p) (silu);
  * weight [d, width], width 2 .. 8.  state [width-1, batch, d] (optional, x's type) = the inputs in front of x (zeros without it);
  * state_out (optional) receives the last width-1 inputs.  Backward: dweight / dbias are written (accumulate = 0) or added to;
- * dstate_out (optional) = gradient of state_out, dstate (optional) receives that of state.  step: one token a sequence,
+ * dstate_out (optional) = gradient of state_out, dstate (optional) receives that of state (over no steps the same).  step: one token a sequence,
  * x [batch, d] with row stride x_b; state_out may be state (updated in place).  At most 65535 sequences of 65535 * 64 steps. */
 int jova_causal_conv_fwd(const void* x, int64_t x_t, int64_t x_b, int dtype, int64_t steps, int64_t batch, int d, int width,
                          const void* weight, const void* bias_or_null, int weight_dtype, int silu,

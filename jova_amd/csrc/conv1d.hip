@@ -194,6 +194,7 @@ conv_bwd_kernel(ConvArgs a) {
     for (; t < min(t1, len) + W - 1; ++t)                // (behind the end: what is left of the last W - 1 gradients)
         one(conv_in<T, W, V>(a, t, b, c, len), t < len ? *(const Pack<T, V>*)(dy + t * a.dy_t + b * a.dy_b + c) : none<T, V>(), t, t < t1, false);
     for (long long s = max(t0, len); s < t1; ++s) *(Pack<T, V>*)(dx + s * dx_t) = none<T, V>();
+    if (!a.part) return;                               // (no steps: the state's gradient only)
     float* part = a.part + ((long long)blockIdx.z * a.batch + b) * (W + 1) * a.d + c;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -333,14 +334,14 @@ extern "C" int jova_causal_conv_bwd(const void* x, int64_t x_t, int64_t x_b, con
     JOVA_CHECK_ARG(weight && dweight && workspace && (steps * batch == 0 || (x && dy && dx)), "causal_conv_bwd: null pointer");
     ConvArgs a = {};
     a.x = x; a.dy = dy; a.weight = weight; a.bias = bias_or_null; a.state = state_or_null; a.dstate_out = dstate_out_or_null;
-    a.dx = dx; a.dstate = dstate_or_null; a.part = (float*)workspace; a.lengths = lengths_or_null;
+    a.dx = dx; a.dstate = dstate_or_null; a.part = steps > 0 ? (float*)workspace : nullptr; a.lengths = lengths_or_null;
     a.x_t = x_t; a.x_b = x_b; a.dy_t = dy_t; a.dy_b = dy_b; a.steps = steps; a.batch = (int)batch; a.d = d; a.silu = silu;
     a.wtype = weight_dtype; a.chunk = BWD_CHUNK;
     const long long chunks = (steps + a.chunk - 1) / a.chunk;
     const hipStream_t s = (hipStream_t)stream;
-    if (steps > 0 && batch > 0) {
+    if (batch > 0 && (steps > 0 || dstate_or_null)) {  // (over no steps the state passes through, and so does its gradient)
         const int v = conv_vec(dtype, BYTES, a), per = 256 * v;
-        const dim3 grid((d + per - 1) / per, (unsigned)batch, (unsigned)chunks);
+        const dim3 grid((d + per - 1) / per, (unsigned)batch, (unsigned)(chunks ? chunks : 1));
         const int rc = conv_dispatch(dtype, width, [&](auto t, auto w) {
             typedef decltype(t) T;
             constexpr int W = decltype(w)::value;
@@ -351,7 +352,7 @@ extern "C" int jova_causal_conv_bwd(const void* x, int64_t x_t, int64_t x_b, con
         });
         if (rc) return rc;
     }
-    hipLaunchKernelGGL(conv_fold_kernel, dim3((d + 63) / 64, width + (dbias_or_null ? 1 : 0)), dim3(1024), 0, s, a.part,
+    hipLaunchKernelGGL(conv_fold_kernel, dim3((d + 63) / 64, width + (dbias_or_null ? 1 : 0)), dim3(1024), 0, s, (const float*)workspace,
                        (long long)(steps > 0 ? chunks * batch : 0), d, width, dweight, dbias_or_null, weight_dtype, accumulate);
     JOVA_CHECK_LAUNCH("causal_conv_bwd (fold)");
     return JOVA_OK;

@@ -921,3 +921,35 @@ def test_scan_backward_whose_chunks_are_cut_into_pieces(device):
     close(h, want[1], mag[1], c, "state")
     for k in keys:                                                   # (the parameters' sums run over the batch too)
         close(got[k], want[2][k], mag[2][k], 2 * c + (t * b if k in ("A", "D", "bias") else 0), "d" + k)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,d,width", [(1, 1, 2), (3, 16, 4), (2, 33, 8), (2, 600, 3)])
+def test_conv_over_no_steps_hands_the_state_and_its_gradient_through(device, b, d, width, dtype):
+    """A piece of zero steps: the state that is returned is the one that came in, and so is its gradient (zeros without one)."""
+    from jova_amd.nn import functional as F
+    g = gen(b + d + width)
+    mk = lambda *s: torch.randn(*s, generator=g).to(dtype).to(device)                                 # noqa: E731
+    x, w, bias, st, ds = mk(5, b, d), mk(d, width), mk(d), mk(width - 1, b, d).requires_grad_(True), mk(width - 1, b, d)
+    pw, pb = w.clone().requires_grad_(True), bias.clone().requires_grad_(True)
+
+    def poison():                                                    # the memory that the next allocation of this size gets
+        torch.full_like(st, float("nan"))
+    for lengths in (None, torch.zeros(b, dtype=torch.int32, device=device)):
+        y, fin = F.causal_conv1d(x[:0], pw, pb, "silu", lengths, st, True)
+        assert y.shape == (0, b, d) and torch.equal(fin, st)
+        poison()
+        got = torch.autograd.grad(fin, (st, pw, pb), ds, retain_graph=True)
+        assert torch.equal(got[0], ds) and float(got[1].abs().max()) == 0.0 and float(got[2].abs().max()) == 0.0
+        poison()
+        got, = torch.autograd.grad(y, st, torch.empty_like(y))
+        assert float(got.abs().max()) == 0.0
+    got = []
+    for cuts in ((0, 3, 5), (0, 0, 3, 3, 5, 5)):                     # pieces of no steps between the others change nothing
+        s = st
+        for lo, hi in zip(cuts, cuts[1:]):
+            y, s = F.causal_conv1d(x[lo:hi], w, bias, "silu", initial_state=s, return_final_state=True)
+            poison()
+        got.append(torch.autograd.grad(s, st, ds)[0])
+    assert torch.equal(got[0], got[1])
