@@ -5,7 +5,8 @@ Every Function's forward/backward only (a) allocates outputs with torch (device 
 
 Parameter gradients: the kernels *accumulate*.  If a parameter already has a ``.grad`` (the trainer keeps all of
 them as views of one flat buffer that it zeroes once per step), the kernels add straight into it and the Function
-returns ``None`` for that input; otherwise a zero tensor is allocated, filled and returned to autograd.
+returns ``None`` for that input; otherwise a zero tensor is allocated, filled and returned to autograd.  The token-sequence
+functions at the end of this file do so only with a ``.grad`` that its owner has marked (``_grad_slot``).
 """
 import array
 import ctypes
@@ -1172,9 +1173,13 @@ def _lengths_i32(who, lengths, x):
 
 
 def _grad_slot(param):
-    """(tensor the kernel writes a parameter's gradient to, accumulate, what backward returns): module docstring."""
+    """(tensor the kernel writes a parameter's gradient to, accumulate, what backward returns).  Only a .grad that its owner has
+    marked (kernels_add: the views of the trainer's flat buffer) is added to in place.  Any other gradient is returned: what
+    torch.autograd.grad was not asked for must not reach .grad, what it was asked for must reach the caller, hooks have to see it,
+    and the engine orders streams behind returned gradients only."""
     g = param.grad if param.is_leaf else None
-    if g is not None and g.dtype == param.dtype and g.device == param.device and g.is_contiguous() and g.data_ptr() % 16 == 0:
+    if (g is not None and getattr(g, "kernels_add", False) and not param._backward_hooks and not param._post_accumulate_grad_hooks
+            and g.dtype == param.dtype and g.device == param.device and g.is_contiguous() and g.data_ptr() % 16 == 0):
         return g, 1, None
     g = torch.empty(param.shape, dtype=param.dtype, device=param.device)
     return g, 0, g
@@ -1215,7 +1220,8 @@ def _workspace(n, like):
 def embedding(idx, weight, scale=1.0, padding_idx=None):
     """scale * weight[idx] (nn.functional.embedding and a multiplication in one pass).  The gradient is summed per token over
     the rows sorted by token, in fp32 and in ascending row order: the same bits on every call, unlike EmbeddingFunction's
-    atomics.  Rows equal to padding_idx give no gradient.  An id outside the table yields a NaN row and is reported by
+    atomics.  Rows equal to padding_idx give no gradient.  (A table whose .grad the trainer's flat buffer owns gets it added there in
+    the backward pass, whatever torch.autograd.grad asks for.)  An id outside the table yields a NaN row and is reported by
     EmbeddingFunction.raise_if_bad()."""
     _check_input("embedding", weight, 2)
     if not torch.is_tensor(idx) or idx.dtype not in (torch.int64, torch.int32):
@@ -1301,7 +1307,8 @@ def _conv_args(who, x, weight, bias, activation, dims):
 def causal_conv1d(x, weight, bias=None, activation=None, lengths=None, initial_state=None, return_final_state=False):
     """Causal depthwise convolution: y[t] = act(bias + sum_k weight[:, k] x[t - width + 1 + k]) for x [steps, batch, dim],
     weight [dim, width] (width 2 .. 8; float32 or x's type), activation None or 'silu'.  initial_state [width-1, batch, dim]
-    holds the inputs in front of x (zeros without it).  Returns y, or (y, final_state) for the next piece of the sequence."""
+    holds the inputs in front of x (zeros without it).  Returns y, or (y, final_state) for the next piece of the sequence.  (As in
+    embedding(), gradients of parameters that the trainer's flat buffer owns are added there.)"""
     who = "causal_conv1d"
     silu = _conv_args(who, x, weight, bias, activation, 3)
     _check_type(who, "initial_state", initial_state, x.dtype, x)

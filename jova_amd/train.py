@@ -164,7 +164,8 @@ def count_parameters(model):
 
 
 class FlatParameters(object):
-    """Re-homes every parameter of ``model`` into one flat fp32 buffer (and every gradient into another)."""
+    """Re-homes every parameter of ``model`` into one flat fp32 buffer (and every gradient into another).  The gradients are
+    marked ``kernels_add``: backward kernels may add to them in place."""
 
     def __init__(self, model):
         params = [p for p in model.parameters() if p.requires_grad]
@@ -182,6 +183,7 @@ class FlatParameters(object):
             self.data[o:o + p.numel()].copy_(p.data.reshape(-1))
             p.data = self.data[o:o + p.numel()].view(p.shape)
             p.grad = self.grad[o:o + p.numel()].view(p.shape)
+            p.grad.kernels_add = True
         self.params, self.n_params, self.numel = params, n, total
 
     def zero_grad(self):

@@ -953,3 +953,57 @@ def test_conv_over_no_steps_hands_the_state_and_its_gradient_through(device, b, 
             poison()
         got.append(torch.autograd.grad(s, st, ds)[0])
     assert torch.equal(got[0], got[1])
+
+
+@pytest.mark.gpu
+def test_gradients_that_nobody_asked_for_leave_an_existing_grad_alone(device):
+    """torch.autograd.grad next to a .grad that is there: what was asked for is returned, .grad stays as it is, hooks see what
+    backward() adds."""
+    from jova_amd.nn import functional as F
+    g = gen(91)
+    x, w, b = (torch.randn(*s, generator=g).to(device).requires_grad_(True) for s in ((20, 2, 12), (12, 4), (12,)))
+    table, idx, dout = torch.randn(9, 12, generator=g).to(device).requires_grad_(True), torch.randint(9, (20, 2), generator=g).to(device), x.detach()
+    calls = {"conv": (lambda: F.causal_conv1d(x, w, b, "silu"), (w, b)), "embedding": (lambda: F.embedding(idx, table), (table,)),
+             "both": (lambda: F.causal_conv1d(F.embedding(idx, table), w, b, "silu"), (table, w, b))}
+    for name, (call, params) in calls.items():
+        for p in params:
+            p.grad = None
+        want = torch.autograd.grad(call(), params, dout)
+        for p in params:
+            p.grad = torch.full_like(p, 3.0)
+        if name == "conv":
+            torch.autograd.grad(call(), x, dout)
+            assert all(float((p.grad - 3.0).abs().max()) == 0.0 for p in params), name
+        got = torch.autograd.grad(call(), params, dout)
+        assert all(torch.equal(p, q) for p, q in zip(got, want)), name
+        assert all(float((p.grad - 3.0).abs().max()) == 0.0 for p in params), name
+        seen, hooks = [], [p.register_hook(lambda v: seen.append(v)) for p in params]
+        at = [p.grad.data_ptr() for p in params]
+        call().backward(dout)
+        for h in hooks:
+            h.remove()
+        assert len(seen) == len(params) and all(torch.is_tensor(v) for v in seen), name
+        assert all(torch.equal(p.grad, q + 3.0) and p.grad.data_ptr() == a for p, q, a in zip(params, want, at)), name
+
+
+@pytest.mark.gpu
+def test_gradients_of_a_flat_buffer_are_added_in_place(device):
+    """The trainer's own gradients (views of FlatParameters' buffer): added to by the kernels, through hooks where there are some."""
+    from jova_amd.nn.layers import CausalConv1d, Embedding
+    from jova_amd.train import FlatParameters
+    torch.manual_seed(7)
+    net = torch.nn.Sequential(Embedding(11, 10, padding_idx=3, scale=2.0), CausalConv1d(10, 3)).to(device)
+    idx = torch.randint(11, (40, 2), generator=gen(92)).to(device)
+    params = list(net.parameters())
+    want = torch.autograd.grad(net(idx).square().sum(), params)
+    flat = FlatParameters(net)
+    flat.grad.fill_(0.5)
+    for trial in range(2):
+        seen = []
+        hooks = [p.register_hook(lambda v: seen.append(v)) for p in params] if trial else []
+        net(idx).square().sum().backward()
+        assert len(seen) == len(hooks) and all(torch.is_tensor(v) for v in seen)
+        for p, q in zip(params, want):
+            assert p.grad.untyped_storage().data_ptr() == flat.grad.untyped_storage().data_ptr()
+            # an addition to 0.5 and one to the first pass's sum: a rounding each of what is there
+            close(p.grad, 0.5 + (trial + 1) * q.double().cpu(), 0.5 + (trial + 1) * q.double().abs().cpu(), 3, "grad")
