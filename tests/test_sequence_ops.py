@@ -1007,3 +1007,24 @@ def test_gradients_of_a_flat_buffer_are_added_in_place(device):
             assert p.grad.untyped_storage().data_ptr() == flat.grad.untyped_storage().data_ptr()
             # an addition to 0.5 and one to the first pass's sum: a rounding each of what is there
             close(p.grad, 0.5 + (trial + 1) * q.double().cpu(), 0.5 + (trial + 1) * q.double().abs().cpu(), 3, "grad")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [2.0, 1.0])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_clip_norm_adds_every_term_in_fp64(device, dtype, kind):
+    """One large value in front of small ones in every 16 bytes: an fp32 sum of the terms would lose each of the small ones (0.9
+    of half a step), together they are 1.35 steps of 2^-24 or more of the norm.  In fp64 the norm takes its last rounding only."""
+    from jova_amd.train import clip_grad_norm_
+    small = 0.9 * U32
+    if dtype == torch.float16 and kind == 1.0:
+        small = 2.0 ** -24                                           # (its least number: exactly half a step, a tie that goes to 1)
+    v = torch.tensor(small if kind == 1.0 else small ** 0.5, dtype=torch.float64).to(dtype)
+    assert float(v) > 0.0 and float(v) ** int(kind) <= U32
+    x = torch.full((3, 16 // v.element_size()), 1.0, dtype=dtype)
+    x[:, 1:] = v
+    for n in (1, 3):
+        for rows in (x[:n], x[:n].repeat(4096, 1)):                  # by single vectors and by whole chunks
+            want = float(rows.double().norm(p=kind))
+            got = float(clip_grad_norm_([rows.to(device)], 1e9, norm_type=kind))
+            assert abs(got - want) <= U32 * want * (1 + 2.0 ** -20), (got, want)
