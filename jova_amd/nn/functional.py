@@ -1566,4 +1566,5 @@ def grad_norm_and_clip(grads, max_norm, kind=2, norm_scale=1.0, out=None):
     ws = _workspace(_lib.lib().jova_clip_grads_workspace_bytes(n), norm)
     _call_on(norm, "jova_clip_grads", n, *[a.buffer_info()[0] for a in (gp, op, sizes, codes)], kind, float(norm_scale), float(max_norm),
              norm.data_ptr(), ws.data_ptr())
+    torch.autograd.graph.increment_version(outs)       # written behind autograd's back: a graph that saved one must notice
     return norm

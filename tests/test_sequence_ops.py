@@ -1028,3 +1028,22 @@ def test_clip_norm_adds_every_term_in_fp64(device, dtype, kind):
             want = float(rows.double().norm(p=kind))
             got = float(clip_grad_norm_([rows.to(device)], 1e9, norm_type=kind))
             assert abs(got - want) <= U32 * want * (1 + 2.0 ** -20), (got, want)
+
+
+@pytest.mark.gpu
+def test_clipping_is_noticed_by_a_graph_that_saved_the_gradient(device):
+    from jova_amd.train import clip_grad_norm_
+    grads = [torch.full((5,), 2.0, device=device), torch.full((3,), 2.0, device=device).half()]
+    outs = [torch.zeros_like(v) for v in grads]
+    clip_grad_norm_(grads, 1.0, out=outs)
+    assert [v._version for v in grads] == [0, 0] and all(v._version > 0 for v in outs)
+    w = torch.ones(5, device=device, requires_grad=True)
+    y = (w * grads[0]).sum()                                         # keeps grads[0] for w's gradient
+    clip_grad_norm_(grads, 1.0)
+    assert all(v._version > 0 for v in grads)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        v = torch.full((4,), 2.0, device=device)
+        clip_grad_norm_([v], 1.0)
+        assert abs(float(v.double().norm()) - 1.0) < 1e-5
