@@ -1193,24 +1193,48 @@ def _wants_grad(*tensors):
     return False
 
 
-_EAGER = []              # weak references to the graphs that eager calls of the functions below have built
+# stream -> weak references to the contexts of the differentiable calls made on it that still live; None: those whose leaves'
+# gradient accumulators may be an earlier graph's, of another stream.  (Copying, adding and discarding are single steps of the
+# interpreter: graphs begin and end on other threads meanwhile.)
+_GRAPHS = {}
+
+
+def _leaves_of(ctx):
+    """Every leaf behind a differentiable call, by identity: its own inputs and those of whatever computed its inputs."""
+    found, seen = {id(t): t for t in ctx.leaves}, set()
+    todo = [n for n, _ in getattr(ctx, "next_functions", ())]
+    while todo:
+        node = todo.pop()
+        if node is None or node in seen:
+            continue
+        seen.add(node)
+        if type(node).__name__ == "AccumulateGrad":
+            found[id(node.variable)] = node.variable
+        todo.extend(n for n, _ in node.next_functions)
+    return found
 
 
 def _note_leaves(ctx, *tensors):
-    """Refuses a forward pass captured into a hipGraph while an eager graph of the same leaves lives that was built on another
-    stream: its gradient accumulators stay on that stream, and the captured backward pass would draw it into the capture, which
-    ends the process."""
-    ctx.stream = torch._C._cuda_getCurrentRawStream(tensors[0].get_device())
-    ctx.leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]
-    if not torch.cuda.is_current_stream_capturing():
-        _EAGER.append(weakref.ref(ctx))
-        if len(_EAGER) & 1023 == 0:
-            _EAGER[:] = [r for r in _EAGER if r() is not None]
-        return
-    alive = [o for o in [r() for r in _EAGER] if o is not None]
-    if any(o.stream != ctx.stream and any(a is b for a in o.leaves for b in ctx.leaves) for o in alive):
-        raise RuntimeError("capturing a differentiable call while an eager graph of the same leaf tensors is alive: drop its "
-                           "results first, or build it on the capture's stream")
+    """Refuses a forward pass captured into a hipGraph while a graph of the same leaves lives that was built on another stream: a
+    leaf's gradient accumulator stays on the stream it was made on as long as any graph holds it, and the captured backward pass would
+    draw that stream into the capture, which ends the process.  Leaves behind other functions count (a parameter's cast, the layers
+    in front); graphs without any of these functions, and leaves that are used only behind them, are not seen."""
+    stream = torch._C._cuda_getCurrentRawStream(tensors[0].get_device())
+    ctx.leaves = [t for t in tensors if t is not None and t.requires_grad and t.is_leaf]     # (the graph keeps them anyway)
+    key, others = stream, [graphs for s, graphs in _GRAPHS.copy().items() if s != stream and graphs]
+    if others:
+        if not torch.cuda.is_current_stream_capturing():
+            key = None                                 # (whether they share leaves is looked at when it matters)
+        else:
+            mine = _leaves_of(ctx)
+            alive = [g for g in [r() for graphs in others for r in graphs.copy()] if g is not None]
+            if any(not mine.keys().isdisjoint(_leaves_of(g)) for g in alive):
+                raise RuntimeError("capturing a differentiable call while an eager graph of the same leaf tensors is alive: drop its "
+                                   "results first, or build it on the capture's stream")
+    graphs = _GRAPHS.get(key)
+    if graphs is None:
+        graphs = _GRAPHS.setdefault(key, set())
+    graphs.add(weakref.ref(ctx, graphs.discard))
 
 
 def _workspace(n, like):

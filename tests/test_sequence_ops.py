@@ -1047,3 +1047,76 @@ def test_clipping_is_noticed_by_a_graph_that_saved_the_gradient(device):
         v = torch.full((4,), 2.0, device=device)
         clip_grad_norm_([v], 1.0)
         assert abs(float(v.double().norm()) - 1.0) < 1e-5
+
+
+class _Noted(torch.autograd.Function):
+    """Stands for a differentiable call of the sequence functions (CPU)."""
+    @staticmethod
+    def forward(ctx, x, w):
+        from jova_amd.nn import functional as F
+        F._note_leaves(ctx, x, w)
+        return x * w
+
+    @staticmethod
+    def backward(ctx, g):
+        return g, g
+
+
+def test_a_capture_over_a_graph_that_holds_the_leaves_by_other_functions_is_refused(monkeypatch):
+    """Parameters behind a cast, an exponential or a product; accumulators that an earlier graph of another stream has made; graphs
+    of other leaves are no hindrance, and nothing is kept of those that have ended, whatever thread made them."""
+    import threading
+    now = threading.local()
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: now.stream, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: now.capturing)
+    x, w, other = torch.ones(2), torch.ones(2, requires_grad=True), torch.ones(2, requires_grad=True)
+
+    def call(stream, w, capturing=False, before=lambda w: w, x=x):
+        now.stream, now.capturing = stream, capturing
+        return _Noted.apply(x, before(w))
+    ways = [lambda w: w, lambda w: w.to(torch.bfloat16), lambda w: -torch.exp(w), lambda w: torch.nn.functional.relu(w * 2.0) + 1.0]
+    for first in ways:
+        for second in ways:
+            eager = call(1, w, before=first)
+            with pytest.raises(RuntimeError, match="eager graph"):
+                call(2, w, True, second)
+            kept = [call(2, other, True, second), call(2, other, True, second)]       # other leaves: twice, with the results alive
+            del eager
+            call(2, w, True, second)
+            del kept
+    # the accumulator of stream 1 lives on in a graph of stream 2, and in one that was built behind that
+    old = call(1, w)
+    new = call(2, w)
+    del old
+    newer = call(2, w)
+    del new
+    with pytest.raises(RuntimeError, match="eager graph"):
+        call(2, w, True)
+    call(2, other, True)
+    del newer
+    warm = call(2, w)
+    call(2, w, True)                                                  # built on the capture's own stream
+    del warm
+    # a captured graph holds its leaves as an eager one does
+    captured = call(2, w, True)
+    with pytest.raises(RuntimeError, match="eager graph"):
+        call(3, w, True)
+    del captured
+    from jova_amd.nn import functional as F
+    assert not any(F._GRAPHS.values())
+
+    def work(k):
+        live = []
+        for i in range(1500):
+            live.append(call(10 + k, w))
+            del live[:len(live) - k - i % 5]
+    held = call(1, w)
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    with pytest.raises(RuntimeError, match="eager graph"):
+        call(2, w, True)
+    del held
+    assert not any(F._GRAPHS.values())
