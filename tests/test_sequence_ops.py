@@ -1120,3 +1120,14 @@ def test_a_capture_over_a_graph_that_holds_the_leaves_by_other_functions_is_refu
         call(2, w, True)
     del held
     assert not any(F._GRAPHS.values())
+
+
+def test_objects_are_built_again_when_the_makefile_changes():
+    """The flags stand in it: objects of other flags must not be linked with new ones."""
+    import os
+    import subprocess
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "jova_amd", "csrc")
+    out = subprocess.run(["make", "-n", "-W", "Makefile", "-C", csrc], check=True, capture_output=True, text=True).stdout
+    sources = sorted(f for f in os.listdir(csrc) if f.endswith(".hip"))
+    compiled = [line for line in out.splitlines() if " -c " in line]
+    assert len(sources) > 0 and all(any(" %s " % s in line for line in compiled) for s in sources), out
