@@ -318,9 +318,11 @@ class ProteinWords(nn.Module):
         off, ln, p_max = input if isinstance(input, tuple) and torch.is_tensor(input[0]) else tab.batch(input, w.device)
         b, vocab = off.shape[0], self.embedding.num_embeddings - 1
         idx = torch.empty((b, p_max, tab.window), dtype=torch.int64, device=w.device)
-        out = torch.empty((p_max, b, tab.window), device=w.device)          # (the kernel's values: one column of the table)
+        # (the kernel's values are not used: it reads one float a word, of the table or, where that is 16 bits wide, of zeros)
+        out = torch.empty((p_max, b, tab.window), device=w.device)
+        column = w.detach() if w.dtype == torch.float32 else torch.zeros(vocab + 1, device=w.device)
         if p_max:
-            F_.call("jova_prot2vec_fwd", F_.P(tab.table), F_.P(off), F_.P(ln), F_.P(w.detach()), b, p_max, tab.window, 1, vocab, 0,
+            F_.call("jova_prot2vec_fwd", F_.P(tab.table), F_.P(off), F_.P(ln), F_.P(column), b, p_max, tab.window, 1, vocab, 0,
                     F_.P(out), F_.P(idx), F_.stream())
         x = self.embedding(idx.transpose(0, 1))
         return x.reshape(p_max, b, -1), ln
@@ -330,7 +332,7 @@ class ProteinSSM(nn.Module):
     """Selective state space protein encoder, next to ProteinRNN: x [P, B, in_dim] (or ProteinWords' pair with the segment
     counts) -> relu(out) [P, B, hidden_dim].  in_proj -> (u, gate); u through a short causal convolution with SiLU; x_proj(u)
     -> time steps, B, C; the scan; out_proj.  No limit on the hidden size, unlike ProteinRNN.  ``step`` extends running
-    sequences by one segment each."""
+    sequences by one segment each.  float32 only, as the Linear layers in it."""
 
     def __init__(self, in_dim, hidden_dim, state_dim=16, conv_width=4, expand=2, dt_rank=None, activation='relu'):
         super(ProteinSSM, self).__init__()
@@ -351,6 +353,14 @@ class ProteinSSM(nn.Module):
         self.D = nn.Parameter(torch.ones(self.inner))
         self.out_proj = Linear(self.inner, self.hidden_dim)
 
+    def _check(self, x):
+        # (Linear reads whatever it is given as fp32: 16-bit rows would be read past their end)
+        if not torch.is_tensor(x) or x.dtype != torch.float32 or self.in_proj.weight.dtype != torch.float32:
+            raise TypeError("ProteinSSM takes float32 inputs and parameters, got %s and %s" % (
+                x.dtype if torch.is_tensor(x) else type(x), self.in_proj.weight.dtype))
+        if x.shape[-1] != self.in_proj.in_features:
+            raise ValueError("ProteinSSM: %d features, got %s" % (self.in_proj.in_features, list(x.shape)))
+
     def _params(self, u):
         r, n = self.dt_rank, self.state_dim
         p = self.x_proj(u)
@@ -359,6 +369,7 @@ class ProteinSSM(nn.Module):
     def forward(self, x, lengths=None):
         if isinstance(x, (tuple, list)):
             x, lengths = x
+        self._check(x)
         h = self.in_proj(x)
         u = self.conv(h[..., :self.inner], lengths=lengths)
         dt, A, B, C = self._params(u)
@@ -372,6 +383,7 @@ class ProteinSSM(nn.Module):
 
     def step(self, x, state):
         """x [B, in_dim], one segment a sequence -> [B, hidden_dim]; ``state`` (new_state) moves on in place."""
+        self._check(x)
         with torch.no_grad():
             h = self.in_proj(x)
             u = self.conv.step(h[..., :self.inner], state[0])

@@ -1131,3 +1131,41 @@ def test_objects_are_built_again_when_the_makefile_changes():
     sources = sorted(f for f in os.listdir(csrc) if f.endswith(".hip"))
     compiled = [line for line in out.splitlines() if " -c " in line]
     assert len(sources) > 0 and all(any(" %s " % s in line for line in compiled) for s in sources), out
+
+
+def test_the_scan_encoder_refuses_what_its_products_would_read_past_the_end():
+    from jova_amd.nn.models import ProteinSSM
+    net = ProteinSSM(6, 8, state_dim=4)
+    x, st = torch.zeros(3, 2, 6), net.new_state(2, "cpu")
+    with pytest.raises((RuntimeError, AssertionError)):
+        net(x)                                                       # (fp32: as far as the products, which want a GPU)
+    for bad in (x.bfloat16(), x.half(), x.double()):
+        with pytest.raises(TypeError, match="float32"):
+            net(bad)
+        with pytest.raises(TypeError, match="float32"):
+            net((bad, torch.tensor([3, 1])))
+        with pytest.raises(TypeError, match="float32"):
+            net.step(bad[0], st)
+    with pytest.raises(ValueError, match="6 features"):
+        net(x[..., :5])
+    with pytest.raises(TypeError, match="float32"):
+        net.bfloat16()(x.bfloat16())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [1, 5])
+def test_protein_words_of_every_type(device, dim, dtype):
+    """Narrow tables too: the ids come from a kernel that reads a float a word."""
+    from jova_amd.nn.models import ProteinWords
+    rng = __import__("numpy").random.RandomState(5)
+    prof = {"P%d" % i: rng.randint(0, 300, size=(n, 3)) for i, n in enumerate((4, 1, 9))}
+    torch.manual_seed(2)
+    words = ProteinWords(prof, 300, dim, scale=2.0).to(dtype).to(device)
+    x, ln = words([("s", "P0"), ("s", "P1"), ("s", "P2")])
+    assert ln.tolist() == [4, 1, 9] and x.dtype == dtype and x.shape == (9, 3, 3 * dim)
+    w = words.embedding.weight.detach().double().cpu()
+    want = torch.zeros(9, 3, 3 * dim, dtype=torch.float64)
+    for i, k in enumerate(prof):
+        want[:prof[k].shape[0], i] = (2.0 * w[torch.from_numpy(prof[k])]).reshape(-1, 3 * dim)
+    assert torch.equal(x.detach().double().cpu(), want)              # (a doubling is exact)
