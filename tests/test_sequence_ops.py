@@ -1169,3 +1169,28 @@ def test_protein_words_of_every_type(device, dim, dtype):
     for i, k in enumerate(prof):
         want[:prof[k].shape[0], i] = (2.0 * w[torch.from_numpy(prof[k])]).reshape(-1, 3 * dim)
     assert torch.equal(x.detach().double().cpu(), want)              # (a doubling is exact)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,b,d,n,gr", [(700, 2, 132, 16, 2), (530, 3, 210, 32, 3), (780, 40, 260, 3, 2)])
+def test_scan_chunks_and_pieces_with_groups_and_channel_tiles(device, t, b, d, n, gr, dtype):
+    """A split time axis in every type, together with groups of several channel tiles (the last ones part empty) and ragged ends; in
+    the last shape the backward pass's chunks are cut into pieces.  Roundings: scan_c, its derivation holds for any split, since
+    a chunk's factor exp(A sum e) takes the place of as many products."""
+    from jova_amd.nn import functional as F
+    g = gen(t + b + d + n)
+    a, dy, dh = scan_inputs(g, t, b, d, n, gr, dtype)
+    lengths = torch.randint(0, t + 1, (b,), generator=g)
+    lengths[:2] = torch.tensor([t, t // 2 + 5])
+    keys = ("x", "dt", "A", "B", "C", "D", "z", "bias", "state")
+    v = {k: a[k].to(device).requires_grad_(True) for k in keys}
+    y, h = F.selective_scan(*(v[k] for k in keys[:8]), True, lengths.to(device), v["state"], True)
+    got = dict(zip(keys, torch.autograd.grad((y, h), [v[k] for k in keys], (dy.to(device), dh.to(device)))))
+    want, mag = (R.scan(*(a[k] for k in keys[:8]), True, lengths, a["state"], dy, dh, mag=m) for m in (False, True))
+    c = scan_c(t, n)
+    close(y, want[0], mag[0], c, "y")
+    close(h, want[1], mag[1], c, "state")
+    for k in keys:
+        extra = {"A": t * b, "D": t * b, "bias": t * b, "B": d // gr, "C": d // gr}.get(k, 0)
+        close(got[k], want[2][k], mag[2][k], 2 * c + extra, "d" + k)
