@@ -375,9 +375,10 @@ enum { JOVA_F32 = 0, JOVA_BF16 = 1, JOVA_F16 = 2 };
  * written as zeros, and the returned state is the one at its end. */
 
 /* out[r][:] = scale * weight[idx[r]][:]; an id outside [0, vocab) sets *bad_flag |= 1 and writes NaN (as jova_embedding_fwd).
- * Backward: dweight[v][:] = scale * sum over { r : idx[r] = v } of dout[r][:] in ascending r, summed in fp32 and rounded
- * once (accumulate = 0: every row of dweight is written, rows without a token as zeros; 1: added to what is there, untouched
- * rows stay).  Rows whose id is padding_idx (-1: none) or outside [0, vocab) add nothing.  No float atomics: the same bits on every call.
+ * Backward: dweight[v][:] = scale * sum over { r : idx[r] = v } of dout[r][:], summed in fp32 and rounded once (accumulate = 0:
+ * every row of dweight is written, rows without a token as zeros; 1: added to what is there, untouched rows stay).  Rows whose
+ * id is padding_idx (-1: none) or outside [0, vocab) add nothing.  No float atomics: r ascending within tiles of 32 sorted rows, the
+ * tiles in an order that shapes and alignment fix, so the same bits on every call of the same shapes and alignment.
  * n, vocab < 2^31 (and n / 32 workgroups within one grid of 2^32 threads); dweight 16-byte aligned.  workspace (16-byte aligned): the bytes that the function names. */
 int jova_token_embedding_fwd(const void* weight, int dtype, const int64_t* idx, int64_t n, int d, int64_t vocab, float scale,
                              void* out, int* bad_flag, void* stream);
@@ -410,6 +411,7 @@ int jova_causal_conv_step(const void* x, int64_t x_b, const void* state, void* s
  * time, batch of x, dt, z; time, batch, group of B, C.  state0 (optional) = h in front of the first step, state_out (optional)
  * = h behind the last.  checkpoints (optional, jova_selective_scan_checkpoint_bytes): states the forward leaves for the backward,
  * one every 8 steps (n_state rounded up to 4, 8, 16, 32).  At most 65535 sequences, a step of at most 2^26 elements (strides too).
+ * An x, e or e x that is not finite may give NaN where the formula gives an infinity.
  * Backward: all gradients are written; dz with z, dD / dbias / dstate0 optional; dB, dC are sums over the group's channels.
  * step: one token a sequence (x [batch, d], B [batch, groups, n_state]; the time strides are ignored); state_out may be state. */
 size_t jova_selective_scan_checkpoint_bytes(int64_t steps, int64_t batch, int d, int n_state);

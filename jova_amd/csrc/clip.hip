@@ -7,7 +7,7 @@
 // by roundings of 2^-53 only.
 // Bound by memory: the gradients are read twice and written once.  The second launch walks every workgroup's chunks backwards, so
 // what the first one read last is still in the 256 MB cache.  400 M bf16 elements in 290 tensors: 471 us for 2.4 GB, 5.1 TB/s.
-// 4 M floats in 48 tensors: 15 us on the card (6.4 + 8.9), 41 us a call: building the tensor table bounds it, on the host.
+// 4 M floats in 48 tensors: 15 us on the card (5.9 + 8.9), 43 us a call: building the tensor table bounds it, on the host.
 #include "seq.h"
 
 #include <algorithm>

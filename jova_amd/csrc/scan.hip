@@ -14,9 +14,11 @@
 // Bound by the vector ALUs, not by memory: per element and state the forward pass has exp (2 issue slots), e A, u B and two
 // multiply-adds, the backward pass about 17 operations, against 8 and 22 bytes per element with 16 states in 16 bits.  Packed fp32
 // operations are not used.  B and C come in through LDS, 16 (8) steps at once, two sides, the next tile's loads in flight meanwhile.
-// 2048 x 8 x 2048, 16 states, bf16: chunk states 110 us (vector ALUs busy 92 %), forward 175 (90 %), chunk adjoints 92 (92 %), backward
-// 447 (86 %).
-// 16384 x 1 x 4096: 500 us, 240 of them chunk states (97 and 96 %).  232 x 128 x 512 ragged fp32: forward 61, backward 149, folds 12 us.
+// 2048 x 8 x 2048, 16 states, bf16: 772 us a call; chunk states 98 (vector ALUs busy 92 %), forward 165 (90 %), chunk adjoints 83 (93 %),
+// backward 398 (86 %), folds 17.  16384 x 1 x 4096: 500 us a call, chunk states 214 (96 %) and forward 285 (97 %).
+// 232 x 128 x 512 ragged fp32: 204 us a call; forward 60, backward 135, folds 12 (vector ALUs busy 80
+// and 77 % of the time that the CUs have work, which is about 70 % of the kernels': lengths differ, no chunks).
+// (Kernels: the fastest of 60 in a trace, whose sums agree with the calls; a trace of 10 ends before the clock has settled.)
 #include "seq.h"
 
 #include <type_traits>
@@ -30,6 +32,8 @@ constexpr int WAVES = 4, CH = 16 * WAVES;              // channels of a workgrou
 // (three waves a SIMD are all its registers allow).
 constexpr int MAX_CHUNKS = 64, FWD_TARGET = 2048, BWD_TARGET = 768;
 // Steps of a chunk at least: with 64, 232 x 128 x 512 (1024 workgroups uncut) would be cut too: 241 against 209 us; 256: no difference.
+// All three constants were swept on the shapes named here.  Few workgroups (one sequence of few channels) run a chunk's 128 steps
+// in series, in up to four passes: a shorter bound for them was not measured.
 constexpr int LEAST_CHUNK = 128;
 // Steps of a tile: the forward passes take 16 (loads, address arithmetic and the barrier are shared by more steps), the backward pass
 // 8, whose states fit the registers of three waves a SIMD; states are saved every 8 steps.  (16 and two waves: 565 against
@@ -433,7 +437,8 @@ scan_adjoint_kernel(ScanArgs a) {
 // instead, 24 permlane swaps and their additions for 4 steps, took 90 issue slots against 32: the vector ALUs bound this kernel.)
 template <int NS> struct Sums {
     static constexpr int NP = 4 * NS, SPLIT = 8 / NS, EACH = 16 / SPLIT;
-    // (16 floats more behind every EACH channels: the SPLIT lanes that read next to each other meet different banks)
+    // (16 floats more behind every EACH channels, for the SPLIT lanes that read next to each other; the whole kernel's counters show
+    // 2.1 M conflict cycles for 17.3 M LDS instructions on 2048 x 8 x 2048, from which access is not known)
     static constexpr int PART = EACH * NP + 16, PITCH = SPLIT * PART;
     float lds[8 * PITCH];
     __device__ __forceinline__ void put(int block, int lane, const float* v) {

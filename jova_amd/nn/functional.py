@@ -1243,8 +1243,8 @@ def _workspace(n, like):
 
 def embedding(idx, weight, scale=1.0, padding_idx=None):
     """scale * weight[idx] (nn.functional.embedding and a multiplication in one pass).  The gradient is summed per token over
-    the rows sorted by token, in fp32 and in ascending row order: the same bits on every call, unlike EmbeddingFunction's
-    atomics.  Rows equal to padding_idx give no gradient.  (A table whose .grad the trainer's flat buffer owns gets it added there in
+    the rows sorted by token, in fp32 and in an order that shapes and alignment fix: the same bits on every such call, unlike
+    EmbeddingFunction's atomics.  Rows equal to padding_idx give no gradient.  (A table whose .grad the trainer's flat buffer owns gets it added there in
     the backward pass, whatever torch.autograd.grad asks for.)  An id outside the table yields a NaN row and is reported by
     EmbeddingFunction.raise_if_bad()."""
     _check_input("embedding", weight, 2)
@@ -1470,7 +1470,8 @@ def selective_scan(x, dt, A, B, C, D=None, z=None, dt_bias=None, dt_softplus=Fal
     """Selective state space scan.  x, dt, z [steps, batch, dim]; B, C [steps, batch, groups, n] or [steps, batch, n]; A [dim, n],
     D and dt_bias [dim] and the states [batch, dim, n] in float32; n <= 32.
         e = dt + dt_bias (softplus of it with dt_softplus);  h[t] = exp(e A) h[t-1] + e x B;  y = (sum_n C h + D x) silu(z)
-    Returns y, or (y, h behind the last step).  Differentiable in everything but lengths."""
+    Returns y, or (y, h behind the last step).  Differentiable in everything but lengths.  An x, e or e x that is not finite
+    may give NaN where the formula gives an infinity (what lies behind a sequence's end is not touched)."""
     who = "selective_scan"
     B, C = _scan_check(who, x, dt, A, B, C, D, z, dt_bias, 3)
     _check_type(who, "initial_state", initial_state, _F32, x)

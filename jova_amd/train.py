@@ -393,8 +393,9 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, norm_scale=1.0, out=Non
     ``parameters``: parameters or other tensors that require a gradient (their ``.grad``; those without one are left out), plain
     tensors that do not (themselves the gradients), or a single one.  norm_type 2, 1 or inf.  norm_scale multiplies the norm
     only (1 / world size where the buffer holds the sum over the ranks and the optimizer divides).  ``out``: tensors that
-    receive the clipped gradients, which then stay as they are.  A norm that is not finite makes the gradients so, as in
-    torch.  No two tensors of the list may share memory."""
+    receive the clipped gradients, which then stay as they are.  As in torch, a norm that is NaN makes every gradient NaN, and an
+    infinite one (or one past fp32's range) makes finite gradients 0 and infinite ones NaN.  No two tensors of the list may share
+    memory; all must be contiguous."""
     kinds = {2.0: 2, 1.0: 1, float("inf"): 0}
     if float(norm_type) not in kinds:
         raise ValueError("clip_grad_norm_: norm_type must be 1, 2 or inf, got %r" % (norm_type,))
