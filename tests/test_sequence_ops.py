@@ -1194,3 +1194,28 @@ def test_scan_chunks_and_pieces_with_groups_and_channel_tiles(device, t, b, d, n
     for k in keys:
         extra = {"A": t * b, "D": t * b, "bias": t * b, "B": d // gr, "C": d // gr}.get(k, 0)
         close(got[k], want[2][k], mag[2][k], 2 * c + extra, "d" + k)
+
+
+@pytest.mark.gpu
+def test_gradients_of_calls_on_another_stream_are_complete_behind_backward(device):
+    """Forward passes on two streams, backward passes called from a third: the caller's stream waits for what they add to .grad."""
+    from jova_amd.nn import functional as F
+    g = gen(93)
+    t, b, d, v = 2000, 8, 256, 500
+    idx, dout = torch.randint(v, (t, b), generator=g).to(device), torch.randn(t, b, d, generator=g).to(device)
+    params = [torch.randn(*s, generator=g).to(device).requires_grad_(True) for s in ((v, d), (d, 4), (d,))]
+
+    def call():
+        return F.causal_conv1d(F.embedding(idx, params[0]), params[1], params[2], "silu")
+    want = torch.autograd.grad(call(), params, dout)
+    for trial in range(5):
+        for p in params:
+            p.grad = torch.zeros_like(p)
+        streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                outs.append(call())
+        for y in outs:
+            y.backward(dout)
+        assert all(torch.equal(p.grad, q + q) for p, q in zip(params, want)), trial
